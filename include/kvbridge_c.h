@@ -210,6 +210,162 @@ typedef struct kvb_append_io {
 const char* kvb_append_shape_error(const kvb_append_shape* s);
 int kvb_append_kv(const kvb_append_shape* s, const kvb_append_io* io, void* stream);
 
+/* ---- 4-bit cache, score forms and eviction (extensions; the reference library
+ * keeps int8 and fp32 caches, knows causal scores only and evicts nothing).
+ *
+ * Cache formats of these calls (kv_bits; dim 64, 128 or 256, page_tokens a
+ * multiple of 8):
+ *   8: the int8 pool of kvb_append_kv; k_scales / v_scales are float.
+ *   4: K and V both token-major, a row of dim / 2 bytes per (page, kv head,
+ *      slot): k[((page * kv_heads + kv) * page_tokens + slot) * (dim / 2) + x].
+ *      A block is 32 consecutive dims; with G = dim / 32, byte n * G + g of a
+ *      row (n = 0..15) holds the codes of dims 32g + 2n (low four bits) and
+ *      32g + 2n + 1.  k_scales / v_scales are G uint32 words per (page, kv
+ *      head, slot), word g = the block's step as bfloat16 in the high half,
+ *      its least value as bfloat16 in the low half: value = code * step + least.
+ * Offsets into the pool are 64 bits wide: a pool may exceed 4 GiB. */
+enum { KVB_OUT_BF16 = 3 };
+
+/* Writes `tokens` new tokens' K and V rows into the 4-bit pool: the shape, the
+ * source rows, the slots and their skipping of ids >= pages * page_tokens are
+ * those of kvb_append_kv.  Per block, in IEEE fp32 (round to nearest even):
+ * least = bf16(min), step = bf16(max(max - least, 0) / 15), code =
+ * clamp(rint((x - least) / step), 0, 15), 0 where step is 0.  A block that
+ * holds a NaN or an infinity, or whose least or step is not finite, is stored
+ * with both NaN and all codes 0.  Two tokens with the same slot race. */
+typedef struct kvb_append_i4_io {
+  const void* k_new;
+  const void* v_new;
+  const uint32_t* slots;
+  uint8_t* k;
+  uint8_t* v;
+  uint32_t* k_scales;
+  uint32_t* v_scales;
+} kvb_append_i4_io;
+const char* kvb_append_i4_shape_error(const kvb_append_shape* s);
+int kvb_append_kv_i4(const kvb_append_shape* s, const kvb_append_i4_io* io, void* stream);
+
+/* Reads the rows of `tokens` slots back as values, k_out / v_out[(t * kv_heads
+ * + kv) * dim + d] in out_type (fp32 product and sum, rounded once); a slot id
+ * >= pages * page_tokens gives a row of zeros. */
+typedef struct kvb_read_shape {
+  uint32_t tokens, kv_heads, dim, page_tokens, pages;
+  uint32_t kv_bits, out_type;
+} kvb_read_shape;
+typedef struct kvb_read_io {
+  const uint32_t* slots;
+  const void* k;
+  const void* v;
+  const void* k_scales;
+  const void* v_scales;
+  void* k_out;
+  void* v_out;
+} kvb_read_io;
+const char* kvb_read_shape_error(const kvb_read_shape* s);
+int kvb_read_kv(const kvb_read_shape* s, const kvb_read_io* io, void* stream);
+
+/* Ragged decode attention over either cache format with score forms.  The
+ * batch metadata is that of kvb_decode_attention_batched (device arrays, every
+ * index clamped).  For query row r of sequence b, head h and key token t
+ *   s = scale * q . k;  cap > 0: s = cap * tanh(s / cap);
+ *   slopes != NULL: s += slopes[h] * (k_position - q_position);
+ *   t is visible when k_position <= q_position and (window == 0 or q_position -
+ *   k_position < window), or when prefix != NULL and k_position < prefix[b].
+ * m = max s, l = sum exp(s - m), out = sum exp(s - m) v / l over the visible
+ * tokens; m = -inf, l = 0, out = 0 where there is none.  What masked tokens
+ * hold, NaN included, has no effect.  Distances of 2^30 and more count as 2^30.
+ * k_positions are nondecreasing within a sequence.
+ * q is [batch][rows][q_heads][dim] of q_type (KVB_SRC_*) with q_stride elements
+ * from one row to the next.  split_tokens is a multiple of 32, or 0 for the
+ * library's choice.  Q of fp32 enters the products as two fp16 digits, the
+ * weights as one (out bf16 from 16-bit q) or two, each scaled by a power of two
+ * per row, and every sum is fp32.
+ * Buffers: kvb_scored_scratch_elements floats; m, l [batch][rows][q_heads];
+ * out [batch][rows][q_heads][dim] in out_type (KVB_OUT_F32, _F16 or _BF16);
+ * counters: NULL (a second launch merges the splits), or
+ * kvb_scored_counter_elements uint32, zero before the first call and left zero
+ * (one launch).  Calls that share scratch or counters must not overlap. */
+typedef struct kvb_scored_shape {
+  uint32_t batch, rows, q_heads, kv_heads, dim, page_tokens, pages;
+  uint32_t max_tokens, total_tokens, table_entries, split_tokens;
+  uint32_t kv_bits, q_type, q_stride, window;
+  float scale, cap;
+} kvb_scored_shape;
+typedef struct kvb_scored_input {
+  const void* q;
+  const int64_t* q_positions;
+  const uint32_t* seq_starts;
+  const uint32_t* page_offsets;
+  const int64_t* k_positions;
+  const uint32_t* page_table;
+  const void* k;
+  const void* v;
+  const void* k_scales;
+  const void* v_scales;
+  const float* slopes;   /* [q_heads] or NULL */
+  const int64_t* prefix; /* [batch] or NULL */
+} kvb_scored_input;
+const char* kvb_scored_shape_error(const kvb_scored_shape* s);
+/* Splits of one sequence (partials in scratch). */
+int kvb_scored_split_count(const kvb_scored_shape* s, uint32_t* splits);
+int kvb_scored_scratch_elements(const kvb_scored_shape* s, size_t* elements);
+int kvb_scored_counter_elements(const kvb_scored_shape* s, size_t* elements);
+int kvb_decode_attention_scored(const kvb_scored_shape* s, const kvb_scored_input* in, float* scratch,
+                                uint32_t* counters, float* m, float* l, void* out, int out_type, void* stream);
+
+/* Attention weights per cached token, with m and l of the call above (the same
+ * shape and input; v, v_scales and split_tokens are not used, v and v_scales
+ * may be NULL): weights[(page * kv_heads + kv) * page_tokens + slot] +=
+ * sum over rows and the kv head's query heads of exp(s - m) / l, 0 where
+ * masked or l is 0.  The last `fresh` tokens of each sequence (those that no
+ * earlier call has counted) are set to that sum instead of added to.  The
+ * adding is atomic: a page in several sequences gets every sequence's sum, in
+ * any order; a page in one sequence gives the same bits in every run. */
+int kvb_accumulate_weights(const kvb_scored_shape* s, const kvb_scored_input* in, const float* m, const float* l,
+                           uint32_t fresh, float* weights, void* stream);
+
+/* Eviction.  Of sequence b's T_b tokens min(T_b, keep) stay: the first `sink`,
+ * the last `recent`, and of the others those with the largest weight, summed
+ * over the kv heads in fp64 and rounded to fp32 (a NaN sum counts as the
+ * least; equal ones: the earlier token).  kvb_evict_select writes their logical
+ * indices, ascending, to kept[b * keep ..] (entries past the count are left as
+ * they are), and kept_starts[b] = tokens kept before sequence b, [batch + 1].
+ * scratch: kvb_evict_scratch_elements uint32.
+ * kvb_evict_move packs the kept tokens into other pages of the same pool: logical
+ * token j of sequence b in the destination is slot j % page_tokens of page
+ * dst_table[dst_offsets[b] + j / page_tokens], and gets codes, scales, the
+ * weight (weights may be NULL) and the position (positions[kept_starts[b] + j],
+ * may be NULL) of token kept[b * keep + j].  kept_starts and positions are then
+ * seq_starts and k_positions of the next call.  A destination page must not be
+ * a page that this call reads, nor occur twice.  Ids >= pages are skipped. */
+typedef struct kvb_evict_shape {
+  uint32_t batch, kv_heads, dim, page_tokens, pages;
+  uint32_t max_tokens, total_tokens, table_entries, dst_entries;
+  uint32_t keep, sink, recent, kv_bits;
+} kvb_evict_shape;
+typedef struct kvb_evict_input {
+  const uint32_t* seq_starts;
+  const uint32_t* page_offsets;
+  const uint32_t* page_table;
+  const int64_t* k_positions;
+} kvb_evict_input;
+typedef struct kvb_evict_cache {
+  void* k;
+  void* v;
+  void* k_scales;
+  void* v_scales;
+  float* weights;
+  const uint32_t* dst_offsets;
+  const uint32_t* dst_table;
+  int64_t* positions;
+} kvb_evict_cache;
+const char* kvb_evict_shape_error(const kvb_evict_shape* s);
+int kvb_evict_scratch_elements(const kvb_evict_shape* s, size_t* elements);
+int kvb_evict_select(const kvb_evict_shape* s, const kvb_evict_input* in, const float* weights, uint32_t* scratch,
+                     uint32_t* kept, uint32_t* kept_starts, void* stream);
+int kvb_evict_move(const kvb_evict_shape* s, const kvb_evict_input* in, const kvb_evict_cache* cache,
+                   const uint32_t* kept, const uint32_t* kept_starts, void* stream);
+
 /* Extension with no counterpart in the reference library, for callers that
  * cannot allocate device memory (code under hipGraph capture, tight serving
  * loops, harnesses that forbid hipMalloc): kvb_decode_attention_fused with its

@@ -22,13 +22,21 @@ from ._capi import (  # noqa: F401
     BatchShape,
     KVB_KERNEL_GENERIC,
     KVB_KERNEL_TILED_MFMA,
+    KVB_OUT_BF16,
     KVB_OUT_F16,
     KVB_OUT_F32,
     KVB_OUT_NONE,
     DeviceInput,
+    EvictCache,
+    EvictInput,
+    EvictShape,
     KvbError,
     KvbInvalidArgument,
     KvbRuntimeError,
+    ReadIO,
+    ReadShape,
+    ScoredInput,
+    ScoredShape,
     Shape,
     check,
     load,
@@ -292,3 +300,130 @@ def append_kv(s: AppendShape, k_new, v_new, slots, k, v, k_scales, v_scales, str
     dim-major."""
     io = AppendIO(*(_ptr(x) for x in (k_new, v_new, slots, k, v, k_scales, v_scales)))
     check(load().kvb_append_kv(ctypes.byref(s), ctypes.byref(io), _stream(stream)))
+
+
+# ---- 4-bit cache: writer and reader (kvb_append_kv_i4, kvb_read_kv) ----------------
+
+def append_i4_shape_error(s: AppendShape):
+    r = load().kvb_append_i4_shape_error(ctypes.byref(s))
+    return None if r is None else r.decode()
+
+
+def append_kv_i4(s: AppendShape, k_new, v_new, slots, k, v, k_scales, v_scales, stream=None) -> None:
+    """Quantize new tokens' K/V rows into their slots of a 4-bit pool
+    (kvb_append_kv_i4): blocks of 32 dims with a bfloat16 step and least value
+    each, K and V token-major."""
+    io = AppendIO(*(_ptr(x) for x in (k_new, v_new, slots, k, v, k_scales, v_scales)))
+    check(load().kvb_append_kv_i4(ctypes.byref(s), ctypes.byref(io), _stream(stream)))
+
+
+def read_shape(tokens, kv_heads, dim, page_tokens, pages, kv_bits=4, out_type: int = KVB_OUT_F32) -> ReadShape:
+    return ReadShape(tokens, kv_heads, dim, page_tokens, pages, kv_bits, out_type)
+
+
+def read_shape_error(s: ReadShape):
+    r = load().kvb_read_shape_error(ctypes.byref(s))
+    return None if r is None else r.decode()
+
+
+def read_kv(s: ReadShape, slots, k, v, k_scales, v_scales, k_out, v_out, stream=None) -> None:
+    """The rows of `slots` as values (kvb_read_kv), [tokens][kv_heads][dim];
+    zeros for slot ids past the pool."""
+    io = ReadIO(*(_ptr(x) for x in (slots, k, v, k_scales, v_scales, k_out, v_out)))
+    check(load().kvb_read_kv(ctypes.byref(s), ctypes.byref(io), _stream(stream)))
+
+
+# ---- attention with score forms over a 4- or 8-bit cache ----------------------------
+
+def make_scored_shape(batch, rows, q_heads, kv_heads, dim, page_tokens, pages, max_tokens, total_tokens, table_entries,
+                      scale, *, kv_bits=4, q_type: int = KVB_SRC_F32, q_stride=None, window=0, cap=0.0,
+                      split_tokens=0) -> ScoredShape:
+    return ScoredShape(batch, rows, q_heads, kv_heads, dim, page_tokens, pages, max_tokens, total_tokens, table_entries,
+                       split_tokens, kv_bits, q_type, q_heads * dim if q_stride is None else q_stride, window,
+                       float(scale), float(cap))
+
+
+def scored_shape_error(s: ScoredShape):
+    r = load().kvb_scored_shape_error(ctypes.byref(s))
+    return None if r is None else r.decode()
+
+
+def scored_split_count(s: ScoredShape) -> int:
+    out = ctypes.c_uint32()
+    check(load().kvb_scored_split_count(ctypes.byref(s), ctypes.byref(out)))
+    return out.value
+
+
+def scored_scratch_elements(s: ScoredShape) -> int:
+    out = ctypes.c_size_t()
+    check(load().kvb_scored_scratch_elements(ctypes.byref(s), ctypes.byref(out)))
+    return out.value
+
+
+def scored_counter_elements(s: ScoredShape) -> int:
+    out = ctypes.c_size_t()
+    check(load().kvb_scored_counter_elements(ctypes.byref(s), ctypes.byref(out)))
+    return out.value
+
+
+def scored_input(q, q_positions, seq_starts, page_offsets, k_positions, page_table, k, v, k_scales, v_scales,
+                 slopes=None, prefix=None) -> ScoredInput:
+    """Build a kvb_scored_input from device tensors (or raw integer pointers)."""
+    return ScoredInput(*(_ptr(x) for x in (q, q_positions, seq_starts, page_offsets, k_positions, page_table,
+                                           k, v, k_scales, v_scales, slopes, prefix)))
+
+
+def decode_attention_scored(s: ScoredShape, inp: ScoredInput, scratch, m, l, out, out_type: int = KVB_OUT_F32,
+                            counters=None, stream=None) -> None:
+    """Ragged decode attention with capped scores, a bias by distance, a window
+    and a visible prefix (kvb_decode_attention_scored)."""
+    check(load().kvb_decode_attention_scored(ctypes.byref(s), ctypes.byref(inp), _ptr(scratch), _ptr(counters), _ptr(m),
+                                             _ptr(l), _ptr(out), out_type, _stream(stream)))
+
+
+def accumulate_weights(s: ScoredShape, inp: ScoredInput, m, l, weights, fresh: int = 0, stream=None) -> None:
+    """Add each cached token's attention weight of a decode_attention_scored
+    call to `weights` [pages][kv_heads][page_tokens] (kvb_accumulate_weights);
+    the last `fresh` tokens of a sequence are set instead."""
+    check(load().kvb_accumulate_weights(ctypes.byref(s), ctypes.byref(inp), _ptr(m), _ptr(l), fresh, _ptr(weights),
+                                        _stream(stream)))
+
+
+# ---- eviction by accumulated weight ---------------------------------------------------
+
+def make_evict_shape(batch, kv_heads, dim, page_tokens, pages, max_tokens, total_tokens, table_entries, dst_entries,
+                     keep, sink=0, recent=0, kv_bits=4) -> EvictShape:
+    return EvictShape(batch, kv_heads, dim, page_tokens, pages, max_tokens, total_tokens, table_entries, dst_entries,
+                      keep, sink, recent, kv_bits)
+
+
+def evict_shape_error(s: EvictShape):
+    r = load().kvb_evict_shape_error(ctypes.byref(s))
+    return None if r is None else r.decode()
+
+
+def evict_scratch_elements(s: EvictShape) -> int:
+    out = ctypes.c_size_t()
+    check(load().kvb_evict_scratch_elements(ctypes.byref(s), ctypes.byref(out)))
+    return out.value
+
+
+def evict_input(seq_starts, page_offsets, page_table, k_positions) -> EvictInput:
+    return EvictInput(*(_ptr(x) for x in (seq_starts, page_offsets, page_table, k_positions)))
+
+
+def evict_cache(k, v, k_scales, v_scales, weights, dst_offsets, dst_table, positions) -> EvictCache:
+    return EvictCache(*(_ptr(x) for x in (k, v, k_scales, v_scales, weights, dst_offsets, dst_table, positions)))
+
+
+def evict_select(s: EvictShape, inp: EvictInput, weights, scratch, kept, kept_starts, stream=None) -> None:
+    """Which tokens of each sequence stay (kvb_evict_select): kept [batch][keep]
+    ascending logical indices, kept_starts [batch + 1]."""
+    check(load().kvb_evict_select(ctypes.byref(s), ctypes.byref(inp), _ptr(weights), _ptr(scratch), _ptr(kept),
+                                  _ptr(kept_starts), _stream(stream)))
+
+
+def evict_move(s: EvictShape, inp: EvictInput, cache: EvictCache, kept, kept_starts, stream=None) -> None:
+    """Pack the kept tokens into the destination pages (kvb_evict_move)."""
+    check(load().kvb_evict_move(ctypes.byref(s), ctypes.byref(inp), ctypes.byref(cache), _ptr(kept), _ptr(kept_starts),
+                                _stream(stream)))

@@ -13,7 +13,7 @@ LIB_NAME = "libkvbridge_amd.so"
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), LIB_NAME)
 
 KVB_OK, KVB_EINVAL, KVB_ERUNTIME = 0, 1, 2
-KVB_OUT_NONE, KVB_OUT_F32, KVB_OUT_F16 = 0, 1, 2
+KVB_OUT_NONE, KVB_OUT_F32, KVB_OUT_F16, KVB_OUT_BF16 = 0, 1, 2, 3
 KVB_KERNEL_TILED_MFMA, KVB_KERNEL_GENERIC = 1, 2
 KVB_SRC_F32, KVB_SRC_F16, KVB_SRC_BF16 = 1, 2, 3
 
@@ -97,6 +97,67 @@ class AppendIO(ctypes.Structure):
     _fields_ = [(n, ctypes.c_void_p) for n in ("k_new", "v_new", "slots", "k", "v", "k_scales", "v_scales")]
 
 
+class ReadShape(ctypes.Structure):
+    """kvb_read_shape (include/kvbridge_c.h)."""
+
+    _fields_ = [(n, ctypes.c_uint32) for n in
+                ("tokens", "kv_heads", "dim", "page_tokens", "pages", "kv_bits", "out_type")]
+
+
+class ReadIO(ctypes.Structure):
+    """kvb_read_io (include/kvbridge_c.h)."""
+
+    _fields_ = [(n, ctypes.c_void_p) for n in ("slots", "k", "v", "k_scales", "v_scales", "k_out", "v_out")]
+
+
+class ScoredShape(ctypes.Structure):
+    """kvb_scored_shape (include/kvbridge_c.h)."""
+
+    _fields_ = [(n, ctypes.c_uint32) for n in
+                ("batch", "rows", "q_heads", "kv_heads", "dim", "page_tokens", "pages", "max_tokens", "total_tokens",
+                 "table_entries", "split_tokens", "kv_bits", "q_type", "q_stride", "window")] + \
+               [("scale", ctypes.c_float), ("cap", ctypes.c_float)]
+
+    def copy(self, **changes) -> "ScoredShape":
+        vals = {f: getattr(self, f) for f, _ in self._fields_}
+        vals.update(changes)
+        return ScoredShape(**vals)
+
+
+class ScoredInput(ctypes.Structure):
+    """kvb_scored_input (include/kvbridge_c.h)."""
+
+    _fields_ = [(n, ctypes.c_void_p) for n in
+                ("q", "q_positions", "seq_starts", "page_offsets", "k_positions", "page_table",
+                 "k", "v", "k_scales", "v_scales", "slopes", "prefix")]
+
+
+class EvictShape(ctypes.Structure):
+    """kvb_evict_shape (include/kvbridge_c.h)."""
+
+    _fields_ = [(n, ctypes.c_uint32) for n in
+                ("batch", "kv_heads", "dim", "page_tokens", "pages", "max_tokens", "total_tokens", "table_entries",
+                 "dst_entries", "keep", "sink", "recent", "kv_bits")]
+
+    def copy(self, **changes) -> "EvictShape":
+        vals = {f: getattr(self, f) for f, _ in self._fields_}
+        vals.update(changes)
+        return EvictShape(**vals)
+
+
+class EvictInput(ctypes.Structure):
+    """kvb_evict_input (include/kvbridge_c.h)."""
+
+    _fields_ = [(n, ctypes.c_void_p) for n in ("seq_starts", "page_offsets", "page_table", "k_positions")]
+
+
+class EvictCache(ctypes.Structure):
+    """kvb_evict_cache (include/kvbridge_c.h)."""
+
+    _fields_ = [(n, ctypes.c_void_p) for n in
+                ("k", "v", "k_scales", "v_scales", "weights", "dst_offsets", "dst_table", "positions")]
+
+
 class KvbError(Exception):
     """Base class; the subclasses mirror std::invalid_argument / std::runtime_error."""
 
@@ -114,6 +175,10 @@ _SP = ctypes.POINTER(Shape)
 _IP = ctypes.POINTER(DeviceInput)
 _BSP = ctypes.POINTER(BatchShape)
 _BIP = ctypes.POINTER(BatchInput)
+_SSP = ctypes.POINTER(ScoredShape)
+_SIP = ctypes.POINTER(ScoredInput)
+_ESP = ctypes.POINTER(EvictShape)
+_EIP = ctypes.POINTER(EvictInput)
 _VP = ctypes.c_void_p
 _U32 = ctypes.c_uint32
 _INT = ctypes.c_int
@@ -153,6 +218,20 @@ SIGNATURES = [
     ("kvb_batch_kernel_name", ctypes.c_char_p, [_BSP, _BIP, _INT]),
     ("kvb_append_shape_error", ctypes.c_char_p, [ctypes.POINTER(AppendShape)]),
     ("kvb_append_kv", _INT, [ctypes.POINTER(AppendShape), ctypes.POINTER(AppendIO), _VP]),
+    ("kvb_append_i4_shape_error", ctypes.c_char_p, [ctypes.POINTER(AppendShape)]),
+    ("kvb_append_kv_i4", _INT, [ctypes.POINTER(AppendShape), ctypes.POINTER(AppendIO), _VP]),
+    ("kvb_read_shape_error", ctypes.c_char_p, [ctypes.POINTER(ReadShape)]),
+    ("kvb_read_kv", _INT, [ctypes.POINTER(ReadShape), ctypes.POINTER(ReadIO), _VP]),
+    ("kvb_scored_shape_error", ctypes.c_char_p, [_SSP]),
+    ("kvb_scored_split_count", _INT, [_SSP, ctypes.POINTER(_U32)]),
+    ("kvb_scored_scratch_elements", _INT, [_SSP, ctypes.POINTER(ctypes.c_size_t)]),
+    ("kvb_scored_counter_elements", _INT, [_SSP, ctypes.POINTER(ctypes.c_size_t)]),
+    ("kvb_decode_attention_scored", _INT, [_SSP, _SIP, _VP, _VP, _VP, _VP, _VP, _INT, _VP]),
+    ("kvb_accumulate_weights", _INT, [_SSP, _SIP, _VP, _VP, _U32, _VP, _VP]),
+    ("kvb_evict_shape_error", ctypes.c_char_p, [_ESP]),
+    ("kvb_evict_scratch_elements", _INT, [_ESP, ctypes.POINTER(ctypes.c_size_t)]),
+    ("kvb_evict_select", _INT, [_ESP, _EIP, _VP, _VP, _VP, _VP, _VP]),
+    ("kvb_evict_move", _INT, [_ESP, _EIP, ctypes.POINTER(EvictCache), _VP, _VP, _VP]),
 ]
 
 _lib = None

@@ -1,0 +1,558 @@
+// Shared parts of the kernels that read a 4- or 8-bit cache under score forms
+// (scored_attend.h, scored_weights.hip): a sequence's extent and the tokens
+// its query rows see, the page lookups of a wave's tiles, and a tile's scores.
+//
+// A tile is 32 tokens, head-rows (query row x query head of one kv head) go in
+// blocks of 16.  Scores are S^T = K Q^T by v_mfma_f32_16x16x32_f16: two
+// products (A, B) of 16 tokens by 16 head-rows for each 32 dims.  The C layout
+// leaves lane (r = l % 16, kg = l / 16) four tokens of A and four of B for
+// head-row r; which tokens those are is the choice of the rows loaded, and is
+// made such that the lane's eight scores are the eight k indices that it has
+// to supply as B operand of O^T = V^T P^T: P never changes lanes.
+//
+// 4 bits, K: a code c in the low bits of a half-word is the fp16 subnormal c *
+// 2^-24, in bits 4..7 it is 16 c * 2^-24, and the products of subnormals are
+// exact here, so a code is unpacked by one mask: two v_perm_b32 and four
+// v_and_b32 give eight of them.  The 2^24 goes into the score's factor, the 16
+// into Q.  A block of 32 dims is one product, so its step multiplies the
+// product's result and its least value the sum of Q over the block: score =
+// sum_g step_g D_g + least_g Qs_g, in fp32.  The codes are not negative and the
+// two terms cancel, and the products' sums are truncated, not rounded, which
+// cost 2e-6 of m and 7e-6 of l; therefore Q's first digit is an integer of 11
+// bits and a sign, with which the sum of 32 products is an exact integer below
+// 2^20, and a second digit holds the rest.
+// 4 bits, V: the same cancellation over a whole context would cost 2e-5 of an
+// output, so codes enter as c - 8 (one v_and_or_b32 and half a v_pk_add_f16 more
+// per two codes) and the block's value at code 8 replaces the least.
+// The block parameters of a lane's tokens lie in the 16 lanes of its row and are
+// read by DPP row broadcasts inside the multiply-adds.
+// 8 bits: codes are converted exactly (i8x8_to_f16), the per-token scale
+// multiplies the sum.
+//
+// Q is scaled by a power of two per head-row such that its largest magnitude
+// lies in [2^13, 2^14).  One digit (8 bits, 16-bit q) then holds it exactly down
+// to 2^-28 of the row's maximum, two within 2^-24 of that maximum.
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include <cfloat>
+#include <cstdint>
+
+#include "device_common.h"
+#include "scored_args.h"
+
+namespace kvb {
+
+typedef uint32_t u32x2_s __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4_s __attribute__((ext_vector_type(4)));
+
+constexpr uint32_t kTileTokens = 32;
+
+// Lane J of each 16-lane row, for folding into the using instruction.  Every
+// lane must be active where it is called: outside of selects and branches.
+template <int J>
+__device__ __forceinline__ float bc(float x) {
+  return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x150 + J, 0xF, 0xF, true));
+}
+template <int J>
+__device__ __forceinline__ int bci(int x) {
+  return __builtin_amdgcn_mov_dpp(x, 0x150 + J, 0xF, 0xF, true);
+}
+
+template <int I, int N, typename F>
+__device__ __forceinline__ void unrolled(F&& f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>{});
+    unrolled<I + 1, N>(f);
+  }
+}
+
+// Sequence b's metadata, every index clamped to the declared sizes.
+struct ScoredSeq {
+  uint32_t start, tokens, table_off;
+};
+__device__ __forceinline__ ScoredSeq clamp_seq(uint32_t s0, uint32_t s1, uint32_t off, uint32_t total, uint32_t entries,
+                                               uint32_t page_tokens, uint32_t max_tokens) {
+  s0 = s0 < total ? s0 : total;
+  s1 = s1 < s0 ? s0 : (s1 < total ? s1 : total);
+  uint32_t t = s1 - s0 < max_tokens ? s1 - s0 : max_tokens;
+  off = off < entries ? off : entries;
+  const uint64_t room = uint64_t(entries - off) * page_tokens;
+  if (t > room) t = uint32_t(room);
+  return ScoredSeq{s0, t, off};
+}
+
+// First t in [0, n) with kpos[t] > x, else n (kpos nondecreasing), by every
+// lane for its own x.  Positions mostly count up by one, so the place that
+// this implies from the last position is tried first: one round of loads
+// instead of a search's seventeen.
+__device__ __forceinline__ uint32_t first_above(const int64_t* __restrict__ kpos, uint32_t n, int64_t last, int64_t x) {
+  if (n == 0u || last <= x) return n;
+  const uint64_t back = uint64_t(last) - uint64_t(x);  // positive
+  uint32_t g = back < n ? n - uint32_t(back) : 0u;
+  const int64_t above = kpos[g], below = g > 0u ? kpos[g - 1u] : INT64_MIN;
+  uint32_t lo = 0, hi = n - 1u;  // kpos[hi] > x
+  if (above > x && (g == 0u || below <= x)) return g;
+  if (above > x) hi = g < hi ? g : hi;
+  else lo = g + 1u;
+  while (lo < hi) {
+    const uint32_t mid = lo + (hi - lo) / 2u;
+    if (kpos[mid] > x) hi = mid;
+    else lo = mid + 1u;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ uint32_t row_min16(uint32_t v) {
+  unrolled<0, 4>([&](auto i) {
+    const uint32_t o = uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x120 + (1 << i), 0xF, 0xF, false));
+    v = o < v ? o : v;
+  });
+  return v;
+}
+__device__ __forceinline__ uint32_t row_max16(uint32_t v) { return ~row_min16(~v); }
+
+// The tokens that head-row r of a block sees: [lo, hi) and [0, pre); and over
+// the block's rows (wave-uniform) the least lo, the largest hi, and the tokens
+// that all of them see: [all_lo, all_hi) or [0, pre).
+struct Visible {
+  uint32_t lo, hi;
+  uint32_t pre, min_lo, max_hi, all_lo, all_hi;
+};
+__device__ __forceinline__ Visible visible_tokens(const ScoredArgs& a, const ScoredSeq& e, uint32_t b, bool valid,
+                                                  int64_t qpos) {
+  Visible v;
+  const int64_t* kpos = a.k_positions + e.start;
+  const int64_t last = e.tokens > 0u ? kpos[e.tokens - 1u] : 0;
+  v.hi = first_above(kpos, e.tokens, last, qpos);
+  v.lo = 0u;
+  if (a.window != 0u) {
+    const int64_t w = int64_t(a.window);
+    // qpos - kpos < window  <=>  kpos > qpos - window
+    if (qpos >= INT64_MIN + w) v.lo = first_above(kpos, e.tokens, last, qpos - w);
+  }
+  if (v.lo > v.hi) v.lo = v.hi;
+  v.pre = 0u;
+  if (a.prefix != nullptr) {
+    const int64_t p = a.prefix[b];
+    if (p > INT64_MIN) v.pre = first_above(kpos, e.tokens, last, p - 1);
+  }
+  if (!valid) v.lo = v.hi = 0u;
+  const bool sees = v.lo < v.hi;
+  v.pre = uint32_t(__builtin_amdgcn_readfirstlane(int(v.pre)));
+  v.min_lo = uint32_t(__builtin_amdgcn_readfirstlane(int(row_min16(sees ? v.lo : 0xffffffffu))));
+  v.max_hi = uint32_t(__builtin_amdgcn_readfirstlane(int(row_max16(sees ? v.hi : 0u))));
+  // A head-row past the last one is never written out: it counts as seeing all.
+  v.all_lo = uint32_t(__builtin_amdgcn_readfirstlane(int(row_max16(valid ? v.lo : 0u))));
+  v.all_hi = uint32_t(__builtin_amdgcn_readfirstlane(int(row_min16(valid ? v.hi : 0xffffffffu))));
+  if (v.max_hi == 0u) v.min_lo = 0u;
+  return v;
+}
+
+// The live tiles of a block: [0, pre_tiles) of the prefix and [first, first +
+// n - pre_tiles) of the rows' windows, numbered 0 .. n - 1.
+struct LiveTiles {
+  uint32_t pre_tiles, first, n;
+  __device__ __forceinline__ uint32_t tile(uint32_t i) const { return i < pre_tiles ? i : i - pre_tiles + first; }
+};
+__device__ __forceinline__ LiveTiles live_tiles(const Visible& v) {
+  LiveTiles t;
+  t.pre_tiles = v.pre / kTileTokens + (v.pre % kTileTokens != 0u ? 1u : 0u);
+  t.first = v.min_lo / kTileTokens;
+  const uint32_t end = v.max_hi / kTileTokens + (v.max_hi % kTileTokens != 0u ? 1u : 0u);
+  if (t.first < t.pre_tiles) t.first = t.pre_tiles;
+  t.n = t.pre_tiles + (end > t.first ? end - t.first : 0u);
+  return t;
+}
+
+// Page and slot of the four runs of 8 tokens of 16 of a wave's tiles: lane l
+// holds run l % 4 of the wave's tile i0 + l / 4 (tile numbers by `tile_of`).
+// Runs past the sequence's end repeat its last one, page ids past the pool the
+// last page, so that every address formed from them lies inside.
+struct TilePages {
+  uint32_t page, slot;
+};
+template <typename F>
+__device__ __forceinline__ TilePages tile_pages(const ScoredArgs& a, const ScoredSeq& e, F tile_of, uint32_t i0,
+                                                uint32_t lane) {
+  const uint32_t last = (e.tokens - 1u) / 8u;
+  const uint64_t run64 = uint64_t(tile_of(i0 + lane / 4u)) * 4u + lane % 4u;
+  const uint32_t run = run64 < last ? uint32_t(run64) : last;
+  const uint32_t per = a.page_tokens / 8u;
+  const uint32_t lp = run / per;
+  const uint32_t page = a.page_table[e.table_off + lp];
+  return TilePages{page < a.pages ? page : a.pages - 1u, (run - lp * per) * 8u};
+}
+
+// A tile's runs, wave-uniform: page and kv head in one number, first slot, and
+// the row number (page, kv head, slot).
+struct TileRows {
+  uint32_t slab[4], slot[4];
+  unsigned long long run[4];
+};
+__device__ __forceinline__ TileRows tile_rows(const ScoredArgs& a, const TilePages& p, uint32_t i, uint32_t kv) {
+  TileRows t;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const uint32_t page = uint32_t(__builtin_amdgcn_readlane(int(p.page), int((i % 16u) * 4u + r)));
+    t.slot[r] = uint32_t(__builtin_amdgcn_readlane(int(p.slot), int((i % 16u) * 4u + r)));
+    t.slab[r] = page * a.kv_heads + kv;
+    t.run[r] = uint64_t(t.slab[r]) * a.page_tokens + t.slot[r];
+  }
+  return t;
+}
+
+// One of four wave-uniform values by the lane's index (values, so that nothing
+// is kept in memory to be indexed).
+template <typename T>
+__device__ __forceinline__ T pick(uint32_t i, T a, T b, T c, T d) {
+  const T lo = (i & 1u) != 0u ? b : a, hi = (i & 1u) != 0u ? d : c;
+  return (i & 2u) != 0u ? hi : lo;
+}
+
+template <int N>
+struct Words {
+  uint32_t w[N];
+};
+// N dwords from p (aligned to them): one load of 4, 8 or 16 bytes, or two.
+template <int N>
+__device__ __forceinline__ Words<N> load_words(const uint8_t* p) {
+  Words<N> r;
+  if constexpr (N == 1) {
+    r.w[0] = *reinterpret_cast<const uint32_t*>(p);
+  } else if constexpr (N == 2) {
+    const u32x2_s v = *reinterpret_cast<const u32x2_s*>(p);
+    r.w[0] = v[0];
+    r.w[1] = v[1];
+  } else {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      const u32x4_s v = reinterpret_cast<const u32x4_s*>(p)[i];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) r.w[4 * i + k] = v[k];
+    }
+  }
+  return r;
+}
+
+__device__ __forceinline__ f16x8 as_f16x8(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __builtin_bit_cast(f16x8, (u32x4_s{a, b, c, d}));
+}
+
+// ---- cache formats: loads and operands of a tile, DIM = 32 G ------------------
+// token(kg, j): the tile's token of index j (0..7) of lane group kg.
+
+template <int G>
+struct Cache4 {
+  static constexpr int kGroups = G;
+  static constexpr int kBits = 4;
+  static constexpr int kVWords = G >= 4 ? G / 4 : 1;
+  static constexpr int kPWords = G / 2;  // parameter words of a lane: word w of a lane group lies in lane w / kPWords
+  struct K {
+    Words<G> a, b;
+    Words<kPWords> p;
+  };
+  struct V {
+    Words<kVWords> v[8];
+    Words<kPWords> p;
+  };
+  static __device__ __forceinline__ uint32_t token(uint32_t kg, uint32_t j) { return 4u * j + kg; }
+
+  // Lane's parameter words: token j = r / 2 of its group, blocks (r % 2) * G / 2 ..
+  static __device__ __forceinline__ Words<kPWords> params(const void* base, const TileRows& t, uint32_t r, uint32_t kg,
+                                                          uint32_t left) {
+    const uint32_t tok = token(kg, r / 2u);
+    const uint64_t row = pick(r / 4u, t.run[0], t.run[1], t.run[2], t.run[3]) + tok % 8u;
+    Words<kPWords> p = load_words<kPWords>(static_cast<const uint8_t*>(base) + row * (4u * G) + (r % 2u) * (2u * G));
+    if (tok >= left) {  // slots behind the sequence hold anything
+#pragma unroll
+      for (int i = 0; i < kPWords; ++i) p.w[i] = 0u;
+    }
+    return p;
+  }
+  // A rows m: tokens 4 (m % 4) + m / 4 of the first 16, B those of the last 16.
+  static __device__ __forceinline__ K load_k(const ScoredArgs& a, const TileRows& t, uint32_t r, uint32_t kg,
+                                             uint32_t left) {
+    const uint32_t in = (4u * (r % 4u) + r / 4u) % 8u;
+    const uint64_t ra = pick(r / 2u % 2u, t.run[0], t.run[1], 0ull, 0ull) + in, rb = pick(r / 2u % 2u, t.run[2], t.run[3], 0ull, 0ull) + in;
+    const uint8_t* base = static_cast<const uint8_t*>(a.k) + kg * (4u * G);
+    K k;
+    k.a = load_words<G>(base + ra * (16u * G));
+    k.b = load_words<G>(base + rb * (16u * G));
+    k.p = params(a.ks, t, r, kg, left);
+    return k;
+  }
+  static __device__ __forceinline__ V load_v(const ScoredArgs& a, const TileRows& t, uint32_t r, uint32_t kg,
+                                             uint32_t left) {
+    V v;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint8_t* p = static_cast<const uint8_t*>(a.v) + (t.run[j / 2] + 4u * (j % 2)) * (16u * G) + kg * (16u * G) + r * G;
+      if constexpr (G == 2) v.v[j].w[0] = *reinterpret_cast<const uint16_t*>(p);
+      else v.v[j] = load_words<kVWords>(p);
+    }
+    v.p = params(a.vs, t, r, kg, left);
+    return v;
+  }
+  // Eight codes of block g, dims 8 kg + (0, 2, 1, 3, 4, 6, 5, 7), the odd dims times 16.
+  template <int g>
+  static __device__ __forceinline__ f16x8 k_frag(const Words<G>& w) {
+    constexpr uint32_t s0 = 0x0c000c00u | uint32_t(g % 4);
+    uint32_t lo, hi;
+    if constexpr (G == 2) {  // bytes g, 2 + g of a dword
+      constexpr uint32_t s = 0x0c000c00u | uint32_t(g) | uint32_t(2 + g) << 16;
+      lo = __builtin_amdgcn_perm(w.w[0], w.w[0], s);
+      hi = __builtin_amdgcn_perm(w.w[1], w.w[1], s);
+    } else {
+      constexpr int at = g / 4, step = G / 4;
+      constexpr uint32_t s = s0 | uint32_t(4 + g % 4) << 16;
+      lo = __builtin_amdgcn_perm(w.w[step + at], w.w[at], s);
+      hi = __builtin_amdgcn_perm(w.w[3 * step + at], w.w[2 * step + at], s);
+    }
+    return as_f16x8(lo & 0x000f000fu, lo & 0x00f000f0u, hi & 0x000f000fu, hi & 0x00f000f0u);
+  }
+  // Dim of Q element j of block g's operand, and whether its code is times 16.
+  static __device__ __forceinline__ uint32_t q_dim(int g, uint32_t kg, int j) {
+    constexpr uint32_t order[8] = {0, 2, 1, 3, 4, 6, 5, 7};
+    return 32u * g + 8u * kg + order[j];
+  }
+  static constexpr bool q_odd(int j) { return (j & 2) != 0; }
+};
+
+template <int G>
+struct Cache8 {
+  static constexpr int kGroups = G;
+  static constexpr int kBits = 8;
+  static constexpr int kPWords = 1;
+  struct K {
+    Words<2 * G> a, b;
+    float p;
+  };
+  struct V {
+    Words<2> v[2 * G];
+    float p;
+  };
+  static __device__ __forceinline__ uint32_t token(uint32_t kg, uint32_t j) { return 8u * kg + j; }
+  // Lanes r and r + 8: the scale of token r % 8 of the group.
+  static __device__ __forceinline__ float params(const float* base, const TileRows& t, uint32_t r, uint32_t kg,
+                                                 uint32_t left) {
+    const uint64_t row = pick(kg, t.run[0], t.run[1], t.run[2], t.run[3]);
+    const float p = base[row + r % 8u];
+    return token(kg, r % 8u) < left ? p : 0.f;
+  }
+  // A rows m: tokens 8 (m / 4) + m % 4, B those four later.
+  static __device__ __forceinline__ K load_k(const ScoredArgs& a, const TileRows& t, uint32_t r, uint32_t kg,
+                                             uint32_t left) {
+    const uint64_t run = pick(r / 4u, t.run[0], t.run[1], t.run[2], t.run[3]);
+    const uint8_t* base = static_cast<const uint8_t*>(a.k) + (run + r % 4u) * (32u * G) + kg * 16u;
+    K k;
+#pragma unroll
+    for (int h = 0; h < G / 2; ++h) {  // 64 dims a piece: 16 bytes of each lane group
+      const Words<4> x = load_words<4>(base + 64u * h), y = load_words<4>(base + 64u * h + 4u * (32u * G));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        k.a.w[4 * h + i] = x.w[i];
+        k.b.w[4 * h + i] = y.w[i];
+      }
+    }
+    k.p = params(static_cast<const float*>(a.ks), t, r, kg, left);
+    return k;
+  }
+  // Dim-major V: dim 16 f + r, the lane group's eight tokens.
+  static __device__ __forceinline__ V load_v(const ScoredArgs& a, const TileRows& t, uint32_t r, uint32_t kg,
+                                             uint32_t left) {
+    const uint32_t slab = pick(kg, t.slab[0], t.slab[1], t.slab[2], t.slab[3]);
+    const uint32_t slot = pick(kg, t.slot[0], t.slot[1], t.slot[2], t.slot[3]);
+    const uint8_t* base = static_cast<const uint8_t*>(a.v) + uint64_t(slab) * (32u * G) * a.page_tokens + slot;
+    V v;
+#pragma unroll
+    for (int f = 0; f < 2 * G; ++f) v.v[f] = load_words<2>(base + uint64_t(16u * f + r) * a.page_tokens);
+    v.p = params(static_cast<const float*>(a.vs), t, r, kg, left);
+    return v;
+  }
+  template <int g>
+  static __device__ __forceinline__ f16x8 k_frag(const Words<2 * G>& w) {
+    return i8x8_to_f16(w.w[2 * g], w.w[2 * g + 1]);
+  }
+  static __device__ __forceinline__ uint32_t q_dim(int g, uint32_t kg, int j) {
+    return 64u * (g / 2) + 16u * kg + 8u * (g % 2) + j;
+  }
+  static constexpr bool q_odd(int) { return false; }
+};
+
+// ---- Q ---------------------------------------------------------------------------
+
+__device__ __forceinline__ float q_element(const void* q, uint64_t i, uint32_t type) {
+  if (type == 1u) return static_cast<const float*>(q)[i];
+  if (type == 2u) return float(static_cast<const _Float16*>(q)[i]);
+  return __uint_as_float(uint32_t(static_cast<const uint16_t*>(q)[i]) << 16);
+}
+
+// Digits of Q: two for 4 bits, and for fp32.
+template <class C, bool F32>
+constexpr int kQDigits = C::kBits == 4 || F32 ? 2 : 1;
+
+// One block's Q operands: fp16 digits of the scaled elements, the sums over
+// each 32 dims (4 bits, in units of 2^-24), and the score's factor.
+template <class C, int QD>
+struct QBlock {
+  f16x8 d[C::kGroups][QD];
+  float sum[C::kBits == 4 ? C::kGroups : 1];
+  float factor;  // score = factor * (sum over dims of the scaled products)
+};
+
+template <class C, int QD>
+__device__ __forceinline__ QBlock<C, QD> load_q(const ScoredArgs& a, uint64_t at, bool valid, uint32_t kg) {
+  constexpr int G = C::kGroups;
+  QBlock<C, QD> q;
+  float x[G][8];
+  float top = 0.f;
+#pragma unroll
+  for (int g = 0; g < G; ++g)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      x[g][j] = valid ? q_element(a.q, at + C::q_dim(g, kg, j), a.q_type) : 0.f;
+      top = fmaxf(top, fabsf(x[g][j]));
+    }
+  top = rows_max(top);
+  int up = 0;  // an infinite or NaN element: the row's result is NaN whatever the scale
+  if (top > 0.f && top <= FLT_MAX) up = 14 - __builtin_amdgcn_frexp_expf(top);  // frexp: top = f * 2^e, f in [1/2, 1)
+  q.factor = ldexpf(a.scale, (C::kBits == 4 ? 24 : 0) - up);
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      float y = ldexpf(x[g][j], up);
+      s += y;
+      if (C::q_odd(j)) y *= 0.0625f;
+      // 4 bits: multiples of 8 up to 2^14 (odd dims: both a 16th)
+      const float unit = C::q_odd(j) ? 0.5f : 8.f;
+      const _Float16 hi = C::kBits == 4 ? _Float16(__builtin_rintf(y * (1.f / unit)) * unit) : _Float16(y);
+      q.d[g][0][j] = hi;
+      if constexpr (QD == 2) q.d[g][1][j] = _Float16(y - float(hi));
+    }
+    if constexpr (C::kBits == 4) q.sum[g] = ldexpf(rows_sum(s), -24);
+  }
+  return q;
+}
+
+// ---- scores ------------------------------------------------------------------------
+
+// The products of a tile: x[j] = sum of step / scale times products plus least
+// value times Q sums, before the score's factor.
+template <class C, int QD>
+__device__ __forceinline__ void tile_scores(const typename C::K& k, const QBlock<C, QD>& q, float (&x)[8]) {
+  constexpr int G = C::kGroups;
+  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+  if constexpr (C::kBits == 4) {
+    constexpr int PW = C::kPWords;
+    float st[PW], le[PW];
+#pragma unroll
+    for (int i = 0; i < PW; ++i) {
+      st[i] = __uint_as_float(k.p.w[i] & 0xffff0000u);
+      le[i] = __uint_as_float(k.p.w[i] << 16);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = 0.f;
+    unrolled<0, G>([&](auto gc) {
+      constexpr int g = gc;
+      const f16x8 ka = C::template k_frag<g>(k.a), kb = C::template k_frag<g>(k.b);
+      f32x4 da = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, q.d[g][0], zero, 0, 0, 0);
+      f32x4 db = __builtin_amdgcn_mfma_f32_16x16x32_f16(kb, q.d[g][0], zero, 0, 0, 0);
+      if constexpr (QD == 2) {
+        da = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, q.d[g][1], da, 0, 0, 0);
+        db = __builtin_amdgcn_mfma_f32_16x16x32_f16(kb, q.d[g][1], db, 0, 0, 0);
+      }
+      unrolled<0, 8>([&](auto jc) {
+        constexpr int j = jc, lane = 2 * j + g / PW, i = g % PW;
+        const float d = j < 4 ? da[j % 4] : db[j % 4];
+        x[j] = fmaf(bc<lane>(st[i]), d, x[j]);
+        x[j] = fmaf(bc<lane>(le[i]), q.sum[g], x[j]);
+      });
+    });
+  } else {
+    f32x4 da = zero, db = zero;
+    unrolled<0, G>([&](auto gc) {
+      constexpr int g = gc;
+      const f16x8 ka = C::template k_frag<g>(k.a), kb = C::template k_frag<g>(k.b);
+#pragma unroll
+      for (int i = 0; i < QD; ++i) {
+        da = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, q.d[g][i], da, 0, 0, 0);
+        db = __builtin_amdgcn_mfma_f32_16x16x32_f16(kb, q.d[g][i], db, 0, 0, 0);
+      }
+    });
+    unrolled<0, 8>([&](auto jc) {
+      constexpr int j = jc;
+      x[j] = bc<j>(k.p) * (j < 4 ? da[j % 4] : db[j % 4]);
+    });
+  }
+}
+
+// cap * tanh(s / cap).  tanh(u) as u times an odd series below 1/4
+// (the next term is under 2^-26 of the value), else 1 - 2 / (e^2u + 1).
+__device__ __forceinline__ float capped(float s, float cap, float inv_cap) {
+  const float u = s * inv_cap, w = u * u;
+  const float series = u * fmaf(w, fmaf(w, fmaf(w, fmaf(w, 0.021869488f, -0.053968254f), 0.13333333f), -0.33333333f), 1.f);
+  const float e = exp_e(2.f * fabsf(u));
+  const float t = copysignf(1.f - 2.f * __builtin_amdgcn_rcpf(e + 1.f), u);
+  return cap * (fabsf(u) < 0.25f ? series : t);
+}
+
+// The distance k_position - q_position in two steps, both clamped to +-2^30:
+// token to the sequence's first row, that row to this one.
+__device__ __forceinline__ int near(int64_t d) {
+  constexpr int64_t kFar = int64_t(1) << 30;
+  return int(d < -kFar ? -kFar : (d > kFar ? kFar : d));
+}
+
+// Score forms on a tile's products: factor, cap, bias by distance, and -inf
+// where MASKED and not visible.  Scores stay in natural units: their difference
+// to a reference is taken first and then multiplied by log2(e) for the
+// exponential.  With the two constants in one rounded factor instead, l of 512
+// tokens was off by 1.1e-6, since every score carried the same relative error.
+struct ScoreForm {
+  float factor, cap, inv_cap, slope;
+  int back;  // this row's position less the first row's
+};
+__device__ __forceinline__ ScoreForm score_form(const ScoredArgs& a, float factor, float slope, int back) {
+  return ScoreForm{factor, a.cap, a.cap > 0.f ? 1.f / a.cap : 0.f, slope, back};
+}
+template <class C, bool MASKED>
+__device__ __forceinline__ void apply_form(const ScoredArgs& a, const ScoreForm& f, int ahead, uint32_t t0, uint32_t kg,
+                                           const Visible& v, float (&x)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) x[j] *= f.factor;
+  if (a.cap > 0.f) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = capped(x[j], f.cap, f.inv_cap);
+  }
+  if (a.slopes != nullptr) {
+    unrolled<0, 8>([&](auto jc) {
+      constexpr int j = jc;
+      x[j] = fmaf(f.slope, float(bci<j>(ahead) - f.back), x[j]);
+    });
+  }
+  if constexpr (MASKED) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t t = t0 + C::token(kg, j);
+      const bool seen = (t >= v.lo && t < v.hi) || t < v.pre;
+      x[j] = seen ? x[j] : neg_inf();
+    }
+  }
+}
+
+// Lane's share of a tile's key positions for the bias by distance: token
+// (kg, r % 8), relative to the first row's position.
+template <class C>
+__device__ __forceinline__ int load_ahead(const ScoredArgs& a, const ScoredSeq& e, uint32_t t0, uint32_t r, uint32_t kg,
+                                          int64_t qref) {
+  if (a.slopes == nullptr) return 0;
+  uint32_t t = t0 + C::token(kg, r % 8u);
+  t = t < e.tokens ? t : e.tokens - 1u;
+  const int64_t p = a.k_positions[e.start + t];
+  return near(int64_t(uint64_t(p) - uint64_t(qref)));
+}
+
+}  // namespace kvb

@@ -1,0 +1,441 @@
+// Ragged decode attention over a 4- or 8-bit cache under score forms
+// (kvb_decode_attention_scored): the split kernel.
+//
+// A work-group of four waves takes one split of (sequence, kv head, block of 16
+// head-rows); its waves take every fourth 32-token tile.  One pass over the
+// tokens with a running reference mref per head-row (not the maximum itself:
+// it moves only when a score exceeds it by 5.5, so that most tiles rescale
+// nothing), l in fp32, and the output's numerators in MFMA
+// accumulators whose column is the head-row, so a rescale is lane-local.
+//
+// PV: the weight of token t for the dims of block g is p_t * step_{t,g}; times
+// 2^ve it enters the product as one fp16 (PD 1: bf16 output, whose step is
+// eight times coarser) or as two (PD 2).  ve is set per head-row where its
+// weights are largest, and again when mref moves or when a step grows by 2^8,
+// which keeps fp16 from overflowing for any steps.  The blocks' values at code
+// 8 add sum_t p_t mid_{t,g} in fp32.
+#pragma once
+#include "scored.h"
+
+namespace kvb {
+
+constexpr int kAttendWaves = 4;
+
+// Partials: (max score, l) pairs of all splits, then the
+// numerators: scratch[(rh * splits + s) * 2], scratch[2 * rh_total * splits +
+// (rh * splits + s) * dim].  l = -1 in split 0: the result is already written.
+struct PartialPlace {
+  float* ml;
+  float* o;
+};
+__device__ __forceinline__ PartialPlace partial_place(const ScoredArgs& a, uint64_t rh, uint32_t split) {
+  const uint64_t all = uint64_t(a.batch) * a.rows * a.q_heads * a.splits;
+  const uint64_t at = rh * a.splits + split;
+  return PartialPlace{a.scratch + at * 2u, a.scratch + all * 2u + at * a.dim};
+}
+
+__device__ __forceinline__ void store_out4(const ScoredArgs& a, uint64_t at, f32x4 o) {
+  if (a.out_type == 1u) {
+    *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + at) = o;
+  } else if (a.out_type == 2u) {
+    typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+    *reinterpret_cast<f16x4*>(static_cast<_Float16*>(a.out) + at) =
+        f16x4{_Float16(o[0]), _Float16(o[1]), _Float16(o[2]), _Float16(o[3])};
+  } else {
+    typedef __bf16 bf16x4_s __attribute__((ext_vector_type(4)));
+    *reinterpret_cast<bf16x4_s*>(static_cast<__bf16*>(a.out) + at) =
+        bf16x4_s{__bf16(o[0]), __bf16(o[1]), __bf16(o[2]), __bf16(o[3])};
+  }
+}
+
+// Running state of a wave: acc[f] columns are head-rows, rows dims.
+template <class C>
+struct AttendState {
+  f32x4 acc[2 * C::kGroups];
+  float mid[C::kBits == 4 ? C::kGroups : 1];
+  float mref, mtop, l, vf;  // reference, maximum of the lane's scores, sum, 2^ve
+  int ve;
+};
+
+// Moves the reference to the head-row's maximum and sets ve by the tile's
+// largest weight.  mult(j): the largest step of the lane's token j.
+template <class C, typename F>
+__device__ __forceinline__ void rescale(AttendState<C>& s, const float (&x)[8], F mult) {
+  const float top = rows_max(s.mtop);
+  const float mref = fmaxf(s.mref, top);
+  const float jump = mref - s.mref;
+  const float alpha = exp_e(-jump);
+  float w = 0.f;
+  unrolled<0, 8>([&](auto jc) {
+    constexpr int j = jc;
+    const float p = exp_e(x[j] - mref), big = mult(jc);
+    w = fmaxf(w, p > 0.f ? p * big : 0.f);
+  });
+  w = rows_max(w);
+  int ve = s.ve;
+  if (w > 0.f && w <= FLT_MAX) {
+    // Upwards only as far as the reference moved: the numerators must not grow.
+    const int room = s.ve + int(fminf(jump * 1.4375f, 200.f));
+    ve = -__builtin_amdgcn_frexp_expf(w);
+    ve = ve < room ? ve : room;
+    ve = ve < -120 ? -120 : (ve > 120 ? 120 : ve);
+  }
+  const int dv = ve - s.ve;
+#pragma unroll
+  for (int f = 0; f < 2 * C::kGroups; ++f)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s.acc[f][i] = ldexpf(s.acc[f][i] * alpha, dv);
+  s.l *= alpha;
+  if constexpr (C::kBits == 4) {
+#pragma unroll
+    for (int g = 0; g < C::kGroups; ++g) s.mid[g] *= alpha;
+  }
+  s.mref = mref;
+  s.ve = ve;
+  s.vf = ldexpf(1.f, ve);
+}
+
+template <int PD>
+struct PDigits {
+  f16x8 d[PD];
+};
+template <int PD>
+__device__ __forceinline__ PDigits<PD> p_digits(const float (&w)[8]) {
+  PDigits<PD> p;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const _Float16 hi = _Float16(w[j]);
+    p.d[0][j] = hi;
+    if constexpr (PD == 2) p.d[1][j] = _Float16(w[j] - float(hi));
+  }
+  return p;
+}
+
+// One tile's weights and their products with V.  MASKED: some head-row does
+// not see every token, whose parameters may be anything.
+template <int G, int PD, bool MASKED>
+__device__ __forceinline__ void tile_values(const ScoredArgs&, const typename Cache4<G>::V& v, const float (&x)[8],
+                                            AttendState<Cache4<G>>& s, uint32_t) {
+  using C = Cache4<G>;
+  constexpr int PW = C::kPWords;
+  float st[PW], mid[PW];
+#pragma unroll
+  for (int i = 0; i < PW; ++i) {
+    st[i] = __uint_as_float(v.p.w[i] & 0xffff0000u);
+    mid[i] = fmaf(st[i], 8.f, __uint_as_float(v.p.w[i] << 16));
+  }
+  float top = 0.f;
+#pragma unroll
+  for (int i = 0; i < PW; ++i) top = fmaxf(top, st[i]);
+  // p < 2^8 and step * 2^ve < 2^7: no weight reaches 2^16
+  if (__any(s.mtop > s.mref + 5.5f) || __any(top * s.vf > 128.f)) {
+    rescale(s, x, [&](auto jc) {
+      constexpr int j = jc;
+      float t = 0.f;
+      unrolled<0, G>([&](auto gc) {
+        constexpr int g = gc, lane = 2 * j + g / PW, i = g % PW;
+        t = fmaxf(t, bc<lane>(st[i]));
+      });
+      return t;
+    });
+  }
+  float p[8], pv[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    p[j] = exp_e(x[j] - s.mref);
+    pv[j] = p[j] * s.vf;
+  }
+  s.l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+  unrolled<0, G>([&](auto gc) {
+    constexpr int g = gc;
+    float w[8];
+    unrolled<0, 8>([&](auto jc) {
+      constexpr int j = jc, lane = 2 * j + g / PW, i = g % PW;
+      const float step = bc<lane>(st[i]), at8 = bc<lane>(mid[i]);
+      if constexpr (MASKED) {
+        const bool in = p[j] != 0.f;
+        w[j] = in ? step * pv[j] : 0.f;
+        s.mid[g] = in ? fmaf(at8, p[j], s.mid[g]) : s.mid[g];
+      } else {
+        w[j] = step * pv[j];
+        s.mid[g] = fmaf(at8, p[j], s.mid[g]);
+      }
+    });
+    const PDigits<PD> d = p_digits<PD>(w);
+    uint32_t u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      constexpr uint32_t sel = 0x0c000c00u | uint32_t(g % 4) | uint32_t(4 + g % 4) << 16;
+      u[i] = __builtin_amdgcn_perm(v.v[2 * i + 1].w[g / 4], v.v[2 * i].w[g / 4], sel);
+    }
+    // 1024 + c and 1024 + 16 c as fp16 bits, less 1032 and 1152
+    f16x8 even = as_f16x8((u[0] & 0x000f000fu) | 0x64006400u, (u[1] & 0x000f000fu) | 0x64006400u,
+                          (u[2] & 0x000f000fu) | 0x64006400u, (u[3] & 0x000f000fu) | 0x64006400u);
+    f16x8 odd = as_f16x8((u[0] & 0x00f000f0u) | 0x64006400u, (u[1] & 0x00f000f0u) | 0x64006400u,
+                         (u[2] & 0x00f000f0u) | 0x64006400u, (u[3] & 0x00f000f0u) | 0x64006400u);
+    even -= (_Float16)1032.f;
+    odd -= (_Float16)1152.f;
+#pragma unroll
+    for (int i = 0; i < PD; ++i) {
+      s.acc[2 * g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, d.d[i], s.acc[2 * g], 0, 0, 0);
+      s.acc[2 * g + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, d.d[i], s.acc[2 * g + 1], 0, 0, 0);
+    }
+  });
+}
+template <int G, int PD, bool MASKED>
+__device__ __forceinline__ void tile_values(const ScoredArgs&, const typename Cache8<G>::V& v, const float (&x)[8],
+                                            AttendState<Cache8<G>>& s, uint32_t) {
+  if (__any(s.mtop > s.mref + 5.5f) || __any(v.p * s.vf > 128.f)) {
+    rescale(s, x, [&](auto jc) {
+      constexpr int j = jc;
+      return bc<j>(v.p);
+    });
+  }
+  float p[8], w[8];
+  unrolled<0, 8>([&](auto jc) {
+    constexpr int j = jc;
+    p[j] = exp_e(x[j] - s.mref);
+    w[j] = bc<j>(v.p) * (p[j] * s.vf);
+    if (MASKED && p[j] == 0.f) w[j] = 0.f;
+  });
+  s.l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+  const PDigits<PD> d = p_digits<PD>(w);
+#pragma unroll
+  for (int f = 0; f < 2 * G; ++f) {
+    const f16x8 c = i8x8_to_f16(v.v[f].w[0], v.v[f].w[1]);
+#pragma unroll
+    for (int i = 0; i < PD; ++i) s.acc[f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(c, d.d[i], s.acc[f], 0, 0, 0);
+  }
+}
+
+// Four consecutive dims of a head-row in units of exp(mref): chunk c of
+// 2 G, and the first of its dims.
+template <int G>
+__device__ __forceinline__ f32x4 chunk_value(const AttendState<Cache4<G>>& s, int c, const float (&mid)[G]) {
+  const int g = c / 2, h = c % 2;
+  const float even = ldexpf(1.f, -s.ve), odd = ldexpf(1.f, -4 - s.ve);
+  return f32x4{fmaf(s.acc[2 * g][2 * h], even, mid[g]), fmaf(s.acc[2 * g + 1][2 * h], odd, mid[g]),
+               fmaf(s.acc[2 * g][2 * h + 1], even, mid[g]), fmaf(s.acc[2 * g + 1][2 * h + 1], odd, mid[g])};
+}
+template <int G>
+__device__ __forceinline__ f32x4 chunk_value(const AttendState<Cache8<G>>& s, int c, const float (&)[1]) {
+  const float f = ldexpf(1.f, -s.ve);
+  return f32x4{s.acc[c][0] * f, s.acc[c][1] * f, s.acc[c][2] * f, s.acc[c][3] * f};
+}
+template <class C>
+__device__ __forceinline__ uint32_t chunk_dim(int c, uint32_t kg) {
+  return C::kBits == 4 ? 32u * (c / 2) + 8u * kg + 4u * (c % 2) : 16u * c + 4u * kg;
+}
+
+template <class C, int QD, int PD>
+__global__ __launch_bounds__(64 * kAttendWaves) void scored_attend_kernel(const ScoredArgs a) {
+  constexpr int G = C::kGroups, NC = 2 * G, NW = kAttendWaves;
+  __shared__ f32x4 lds_o[NW][NC][64];
+  __shared__ float lds_m[NW][16], lds_l[NW][16];
+  const uint32_t lane = threadIdx.x & 63u, r = lane & 15u, kg = lane >> 4;
+  const uint32_t wave = uint32_t(__builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6)));
+  uint32_t at = blockIdx.x;
+  const uint32_t kv = at % a.kv_heads;
+  at /= a.kv_heads;
+  const uint32_t block = at % a.blocks;
+  at /= a.blocks;
+  const uint32_t split = at % a.splits, b = at / a.splits;
+
+  const uint32_t hr = block * 16u + r;
+  const bool valid = hr < a.head_rows;
+  const uint32_t hrc = valid ? hr : a.head_rows - 1u;
+  const uint32_t row = hrc / a.group, head = kv * a.group + hrc % a.group;
+  const uint64_t rh = (uint64_t(b) * a.rows + row) * a.q_heads + head;
+  const ScoredSeq e = clamp_seq(a.seq_starts[b], a.seq_starts[b + 1u], a.page_offsets[b], a.total_tokens, a.table_entries,
+                                a.page_tokens, a.max_tokens);
+  const int64_t qref = a.q_positions[uint64_t(b) * a.rows], qpos = a.q_positions[uint64_t(b) * a.rows + row];
+  const Visible vis = visible_tokens(a, e, b, valid, qpos);
+  const LiveTiles live = live_tiles(vis);
+  uint32_t per = live.n / a.splits + (live.n % a.splits != 0u ? 1u : 0u);
+  per = per > a.split_tiles ? per : a.split_tiles;
+  const uint32_t own = live.n > 0u ? (live.n - 1u) / per + 1u : 1u;
+  if (split >= own) {
+    if (a.splits > 1u && wave == 0u && valid && kg == 0u) {
+      float* ml = partial_place(a, rh, split).ml;
+      ml[0] = neg_inf();
+      ml[1] = 0.f;
+    }
+    return;
+  }
+
+  const uint64_t q_at = (uint64_t(b) * a.rows + row) * a.q_stride + uint64_t(head) * a.dim;
+  const QBlock<C, QD> q = load_q<C, QD>(a, q_at, valid, kg);
+  const ScoreForm form = score_form(a, q.factor, a.slopes ? a.slopes[head] : 0.f, near(int64_t(uint64_t(qpos) - uint64_t(qref))));
+
+  AttendState<C> s;
+#pragma unroll
+  for (int f = 0; f < NC; ++f) s.acc[f] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int g = 0; g < (C::kBits == 4 ? G : 1); ++g) s.mid[g] = 0.f;
+  s.mref = -FLT_MAX;
+  s.mtop = neg_inf();
+  s.l = 0.f;
+  s.vf = 1.f;
+  s.ve = 0;
+
+  const uint32_t first = split * per + wave;
+  const uint32_t end = live.n - split * per > per ? split * per + per : live.n;
+  const uint32_t n = first < end ? (end - first + NW - 1u) / NW : 0u;
+  const auto tile_of = [&](uint32_t i) {
+    const uint64_t t = uint64_t(first) + uint64_t(i) * NW;
+    return live.tile(t < live.n ? uint32_t(t) : live.n - 1u);
+  };
+  if (n > 0u) {
+    TilePages pages = tile_pages(a, e, tile_of, 0u, lane), ahead_pages = pages;
+    TileRows rows = tile_rows(a, pages, 0u, kv);
+    uint32_t t0 = tile_of(0u) * kTileTokens;
+    typename C::K k = C::load_k(a, rows, r, kg, e.tokens - t0);
+    int ahead = load_ahead<C>(a, e, t0, r, kg, qref);
+    for (uint32_t i = 0; i < n; ++i) {
+      if (i % 16u == 0u) ahead_pages = tile_pages(a, e, tile_of, i + 16u, lane);  // a window ahead
+      const typename C::V v = C::load_v(a, rows, r, kg, e.tokens - t0);
+      const uint32_t t_next = tile_of(i + 1u < n ? i + 1u : i) * kTileTokens;
+      if ((i + 1u) % 16u == 0u) pages = ahead_pages;
+      const TileRows rows_next = tile_rows(a, pages, i + 1u < n ? i + 1u : i, kv);
+      const typename C::K k_next = C::load_k(a, rows_next, r, kg, e.tokens - t_next);
+      const int ahead_next = load_ahead<C>(a, e, t_next, r, kg, qref);
+      float x[8];
+      tile_scores<C, QD>(k, q, x);
+      const bool whole = t0 + kTileTokens <= vis.pre || (t0 >= vis.all_lo && t0 + kTileTokens <= vis.all_hi);
+      const auto tops = [&] {
+        s.mtop = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])), s.mtop));
+      };
+      if (whole) {
+        apply_form<C, false>(a, form, ahead, t0, kg, vis, x);
+        tops();
+        tile_values<G, PD, false>(a, v, x, s, kg);
+      } else {
+        apply_form<C, true>(a, form, ahead, t0, kg, vis, x);
+        tops();
+        tile_values<G, PD, true>(a, v, x, s, kg);
+      }
+      k = k_next;
+      rows = rows_next;
+      t0 = t_next;
+      ahead = ahead_next;
+    }
+  }
+
+  // The waves' parts: a common maximum, then each wave adds a quarter of the dims.
+  const float l = rows_sum(s.l), mtop = rows_max(s.mtop);
+  if (kg == 0u) lds_m[wave][r] = mtop;
+  float mid[C::kBits == 4 ? G : 1];
+#pragma unroll
+  for (int g = 0; g < (C::kBits == 4 ? G : 1); ++g) mid[g] = rows_sum(s.mid[g]);
+  __syncthreads();
+  float top = lds_m[0][r];
+#pragma unroll
+  for (int w = 1; w < NW; ++w) top = fmaxf(top, lds_m[w][r]);
+  // A wave without visible tokens has mref = -FLT_MAX: a factor of 0.
+  const float f = l == 0.f ? 0.f : exp_e(s.mref - top);
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    f32x4 o = chunk_value(s, c, mid);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = l == 0.f ? 0.f : o[i] * f;
+    lds_o[wave][c][lane] = o;
+  }
+  if (kg == 0u) lds_l[wave][r] = l * f;
+  __syncthreads();
+  float sum = lds_l[0][r];
+#pragma unroll
+  for (int w = 1; w < NW; ++w) sum += lds_l[w][r];
+  const bool done = own == 1u;
+  const PartialPlace part = done ? PartialPlace{nullptr, nullptr} : partial_place(a, rh, split);
+#pragma unroll
+  for (int i = 0; i < NC / NW; ++i) {
+    const int c = wave * (NC / NW) + i;
+    f32x4 o = lds_o[0][c][lane];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) o += lds_o[w][c][lane];
+    if (!valid) continue;
+    const uint32_t d = chunk_dim<C>(c, kg);
+    if (done) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) o[k] = sum == 0.f ? 0.f : o[k] / sum;
+      store_out4(a, rh * a.dim + d, o);
+    } else {
+      *reinterpret_cast<f32x4*>(part.o + d) = o;
+    }
+  }
+  if (wave == 0u && valid && kg == 0u) {
+    if (done) {
+      a.m[rh] = sum == 0.f ? neg_inf() : top;
+      a.l[rh] = sum;
+      if (a.splits > 1u) partial_place(a, rh, 0u).ml[1] = -1.f;
+    } else {
+      part.ml[0] = top;
+      part.ml[1] = sum;
+    }
+  }
+}
+
+// The joint result of a head-row's splits: one work-group of dim threads times
+// 256 / dim groups of splits per head-row.
+template <int DIM>
+__global__ __launch_bounds__(256) void scored_merge_kernel(const ScoredArgs a) {
+  constexpr int GR = 256 / (DIM / 4);  // groups of splits
+  __shared__ f32x4 lds_o[GR][DIM / 4];
+  __shared__ float lds_l[GR];
+  const uint64_t rh = blockIdx.x;
+  const PartialPlace p = partial_place(a, rh, 0u);
+  if (p.ml[1] == -1.f) return;
+  const uint32_t quad = threadIdx.x % (DIM / 4), gr = threadIdx.x / (DIM / 4), lane = threadIdx.x & 63u;
+  float top = neg_inf();
+  for (uint32_t j = lane; j < a.splits; j += 64u) top = fmaxf(top, p.ml[2u * j]);
+  top = wave_max(top);
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  float l = 0.f;
+  for (uint32_t j = gr; j < a.splits; j += GR) {
+    const float lj = p.ml[2u * j + 1u];
+    if (lj == 0.f) continue;
+    const float f = exp_e(p.ml[2u * j] - top);
+    l += lj * f;
+    o += *reinterpret_cast<const f32x4*>(p.o + uint64_t(j) * DIM + 4u * quad) * f;
+  }
+  lds_o[gr][quad] = o;
+  if (quad == 0u) lds_l[gr] = l;
+  __syncthreads();
+  if (gr != 0u) return;
+#pragma unroll
+  for (int g = 1; g < GR; ++g) {
+    o += lds_o[g][quad];
+    l += lds_l[g];
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) o[k] = l == 0.f ? 0.f : o[k] / l;
+  store_out4(a, rh * DIM + 4u * quad, o);
+  if (quad == 0u) {
+    a.m[rh] = l == 0.f ? neg_inf() : top;
+    a.l[rh] = l;
+  }
+}
+
+template <class C, int QD, int PD>
+inline hipError_t launch_attend_kernel(const ScoredArgs& a, hipStream_t stream) {
+  const uint32_t groups = a.batch * a.splits * a.blocks * a.kv_heads;
+  scored_attend_kernel<C, QD, PD><<<groups, 64 * kAttendWaves, 0, stream>>>(a);
+  return hipGetLastError();
+}
+// Weights of one digit only where the output is bf16 and q has 16 bits.
+template <class C>
+inline hipError_t launch_attend_cache(const ScoredArgs& a, hipStream_t stream) {
+  if (a.q_type == 1u) return launch_attend_kernel<C, 2, 2>(a, stream);
+  constexpr int QD = kQDigits<C, false>;
+  if (a.out_type == 3u) return launch_attend_kernel<C, QD, 1>(a, stream);
+  return launch_attend_kernel<C, QD, 2>(a, stream);
+}
+
+hipError_t launch_attend4_d64(const ScoredArgs& a, hipStream_t stream);
+hipError_t launch_attend4_d128(const ScoredArgs& a, hipStream_t stream);
+hipError_t launch_attend4_d256(const ScoredArgs& a, hipStream_t stream);
+hipError_t launch_attend8_d64(const ScoredArgs& a, hipStream_t stream);
+hipError_t launch_attend8_d128(const ScoredArgs& a, hipStream_t stream);
+hipError_t launch_attend8_d256(const ScoredArgs& a, hipStream_t stream);
+
+}  // namespace kvb

@@ -1,0 +1,8 @@
+// 4-bit cache, head size 256 (scored_attend.h).
+#include "scored_attend.h"
+
+namespace kvb {
+hipError_t launch_attend4_d256(const ScoredArgs& a, hipStream_t stream) {
+  return launch_attend_cache<Cache4<8>>(a, stream);
+}
+}  // namespace kvb

@@ -1,0 +1,8 @@
+// 8-bit cache, head size 64 (scored_attend.h).
+#include "scored_attend.h"
+
+namespace kvb {
+hipError_t launch_attend8_d64(const ScoredArgs& a, hipStream_t stream) {
+  return launch_attend_cache<Cache8<2>>(a, stream);
+}
+}  // namespace kvb

@@ -1,0 +1,107 @@
+// Validation and sizing of the calls on a 4- or 8-bit cache (host only, no
+// HIP): the writer and reader, the scored attention and weights, eviction.
+#include "scored_shape.h"
+
+#include <cmath>
+#include <limits>
+
+namespace kvb {
+namespace {
+
+// Threads of a grid dimension are counted in 32 bits, and work-groups have 256.
+constexpr uint64_t kMaxGroups = (uint64_t(1) << 24) - 1;
+
+const char* cache_error(uint32_t kv_heads, uint32_t dim, uint32_t page_tokens, uint32_t pages, uint32_t kv_bits) {
+  if (kv_bits != 4 && kv_bits != 8) return "kv_bits must be 4 or 8";
+  if (dim != 64 && dim != 128 && dim != 256) return "dim must be 64, 128 or 256";
+  if (page_tokens == 0 || page_tokens % 8 != 0) return "page_tokens must be a positive multiple of 8";
+  if (pages == 0) return "pages must be positive";
+  if (kv_heads == 0 || kv_heads > 65535) return "kv_heads must be in [1,65535]";
+  if (uint64_t(pages) * kv_heads > 0xffffffffull) return "page and kv head product exceeds 32 bits";
+  return nullptr;
+}
+
+uint32_t ceil_div(uint64_t a, uint64_t b) { return uint32_t((a + b - 1) / b); }
+
+}  // namespace
+
+const char* append4_error(const kvb_append_shape& s) {
+  if (const char* e = cache_error(s.kv_heads, s.dim, s.page_tokens, s.pages, 4)) return e;
+  if (s.src_type != KVB_SRC_F32 && s.src_type != KVB_SRC_F16 && s.src_type != KVB_SRC_BF16)
+    return "unknown source element type";
+  if (uint64_t(s.k_stride) < uint64_t(s.kv_heads) * s.dim || uint64_t(s.v_stride) < uint64_t(s.kv_heads) * s.dim)
+    return "token stride must cover kv_heads * dim elements";
+  if ((uint64_t(s.tokens) * s.kv_heads + 63) / 64 > kMaxGroups) return "token and kv head product exceeds the grid limit";
+  return nullptr;
+}
+
+const char* read_error(const kvb_read_shape& s) {
+  if (const char* e = cache_error(s.kv_heads, s.dim, s.page_tokens, s.pages, s.kv_bits)) return e;
+  if (s.out_type != KVB_OUT_F32 && s.out_type != KVB_OUT_F16 && s.out_type != KVB_OUT_BF16) return "unknown output type";
+  if ((uint64_t(s.tokens) * s.kv_heads + 63) / 64 > kMaxGroups) return "token and kv head product exceeds the grid limit";
+  return nullptr;
+}
+
+uint32_t scored_blocks(const kvb_scored_shape& s) { return ceil_div(uint64_t(s.rows) * (s.q_heads / s.kv_heads), 16); }
+
+// Work-groups of the attention: two fit a CU, and a split of fewer than 16
+// tiles (four per wave) is not worth its merge.  Where the caller names no
+// split the tokens that a row can see are cut such that about four rounds of
+// work-groups fill 256 CUs, at most 128 per sequence.
+ScoredSplits scored_splits(const kvb_scored_shape& s) {
+  const uint64_t seen = s.window == 0 ? s.max_tokens
+                                      : std::min<uint64_t>(s.max_tokens, uint64_t(s.window) + s.rows + 32);
+  const uint64_t tiles = (seen + 31) / 32;
+  uint64_t per = s.split_tokens / 32;
+  if (per == 0) {
+    const uint64_t others = uint64_t(s.batch) * s.kv_heads * scored_blocks(s);
+    const uint64_t splits = std::max<uint64_t>(1, std::min<uint64_t>(128, 2048 / others));
+    per = std::max<uint64_t>(16, (tiles + splits - 1) / splits);
+  }
+  return ScoredSplits{uint32_t(std::max<uint64_t>(1, (tiles + per - 1) / per)), uint32_t(per)};
+}
+
+const char* scored_error(const kvb_scored_shape& s) {
+  if (s.batch == 0 || s.batch > 65535) return "batch must be in [1,65535]";
+  if (s.rows == 0 || s.q_heads == 0 || s.kv_heads == 0) return "rows and head counts must be positive";
+  if (s.q_heads % s.kv_heads != 0) return "q_heads must be divisible by kv_heads";
+  if (const char* e = cache_error(s.kv_heads, s.dim, s.page_tokens, s.pages, s.kv_bits)) return e;
+  if (s.max_tokens == 0 || s.max_tokens > 0x7fffffffu) return "max_tokens must be in [1,2^31-1]";
+  if (uint64_t(s.max_tokens) > uint64_t(s.pages) * s.page_tokens) return "tokens exceed allocated page capacity";
+  if (s.total_tokens == 0 || s.table_entries == 0) return "total_tokens and table_entries must be positive";
+  if (s.split_tokens % 32 != 0) return "split_tokens must be a multiple of 32";
+  if (s.q_type != KVB_SRC_F32 && s.q_type != KVB_SRC_F16 && s.q_type != KVB_SRC_BF16) return "unknown query element type";
+  if (uint64_t(s.q_stride) < uint64_t(s.q_heads) * s.dim) return "row stride must cover q_heads * dim elements";
+  if (!std::isfinite(s.scale)) return "score scale must be finite";
+  if (!std::isfinite(s.cap) || s.cap < 0.f) return "score cap must be finite and not negative";
+  if (uint64_t(s.rows) * s.q_heads > kMaxGroups || uint64_t(s.batch) * s.rows * s.q_heads > kMaxGroups)
+    return "batch row/head product exceeds the grid limit";
+  const ScoredSplits p = scored_splits(s);
+  if (p.splits > 65535) return "split count exceeds 65535";
+  if (uint64_t(s.batch) * s.kv_heads * scored_blocks(s) * p.splits > kMaxGroups)
+    return "split and head product exceeds the grid limit";
+  return nullptr;
+}
+
+const char* evict_error(const kvb_evict_shape& s) {
+  if (s.batch == 0 || s.batch > 65535) return "batch must be in [1,65535]";
+  if (const char* e = cache_error(s.kv_heads, s.dim, s.page_tokens, s.pages, s.kv_bits)) return e;
+  if (s.max_tokens == 0 || s.max_tokens > 0x7fffffffu) return "max_tokens must be in [1,2^31-1]";
+  if (s.total_tokens == 0 || s.table_entries == 0 || s.dst_entries == 0)
+    return "total_tokens, table_entries and dst_entries must be positive";
+  if (s.keep == 0 || s.keep > (1u << 30)) return "keep must be in [1,2^30]";
+  if (uint64_t(s.sink) + s.recent > s.keep) return "sink and recent exceed keep";
+  if (uint64_t(s.batch) * s.keep > 0xffffffffull) return "batch and keep product exceeds 32 bits";
+  return nullptr;
+}
+
+// Tiles per work-group of the weights: four per wave, more where the grid
+// would otherwise hold over 4096 work-groups.
+ScoredChunks scored_chunks(const kvb_scored_shape& s) {
+  const uint64_t tiles = (uint64_t(s.max_tokens) + 31) / 32, others = uint64_t(s.batch) * s.kv_heads;
+  const uint64_t most = std::max<uint64_t>(1, 4096 / others);
+  const uint64_t per = std::max<uint64_t>(16, (tiles + most - 1) / most);
+  return ScoredChunks{uint32_t((tiles + per - 1) / per), uint32_t(per)};
+}
+
+}  // namespace kvb

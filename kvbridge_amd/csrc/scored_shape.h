@@ -1,0 +1,28 @@
+// Validation and sizing of the calls on a 4- or 8-bit cache; host only.
+#pragma once
+#include <algorithm>
+#include <cstdint>
+
+#include "kvbridge_c.h"
+
+namespace kvb {
+
+// nullptr when valid, else the first failed rule's message.
+const char* append4_error(const kvb_append_shape& s);
+const char* read_error(const kvb_read_shape& s);
+const char* scored_error(const kvb_scored_shape& s);
+const char* evict_error(const kvb_evict_shape& s);
+
+uint32_t scored_blocks(const kvb_scored_shape& s);  // blocks of 16 head-rows per kv head
+
+struct ScoredSplits {
+  uint32_t splits, tiles;  // partials per sequence, least tiles of a split
+};
+ScoredSplits scored_splits(const kvb_scored_shape& s);
+
+struct ScoredChunks {
+  uint32_t chunks, tiles;  // work-groups per sequence and kv head, tiles of each
+};
+ScoredChunks scored_chunks(const kvb_scored_shape& s);
+
+}  // namespace kvb
