@@ -185,19 +185,24 @@ __device__ __forceinline__ TilePages tile_pages(const ScoredArgs& a, const Score
 }
 
 // A tile's runs, wave-uniform: page and kv head in one number, first slot, and
-// the row number (page, kv head, slot).
+// the row number (page, kv head, slot).  ONE: pages hold whole tiles, so that
+// the four runs follow each other and only the first is kept.
+template <bool ONE>
 struct TileRows {
-  uint32_t slab[4], slot[4];
-  unsigned long long run[4];
+  static constexpr int kRuns = ONE ? 1 : 4;
+  uint32_t slab[kRuns], slot[kRuns];
+  __device__ __forceinline__ uint64_t row(int i, uint32_t page_tokens) const {
+    return uint64_t(slab[ONE ? 0 : i]) * page_tokens + slot[ONE ? 0 : i] + (ONE ? 8u * uint32_t(i) : 0u);
+  }
 };
-__device__ __forceinline__ TileRows tile_rows(const ScoredArgs& a, const TilePages& p, uint32_t i, uint32_t kv) {
-  TileRows t;
+template <bool ONE>
+__device__ __forceinline__ TileRows<ONE> tile_rows(const ScoredArgs& a, const TilePages& p, uint32_t i, uint32_t kv) {
+  TileRows<ONE> t;
 #pragma unroll
-  for (int r = 0; r < 4; ++r) {
+  for (int r = 0; r < TileRows<ONE>::kRuns; ++r) {
     const uint32_t page = uint32_t(__builtin_amdgcn_readlane(int(p.page), int((i % 16u) * 4u + r)));
     t.slot[r] = uint32_t(__builtin_amdgcn_readlane(int(p.slot), int((i % 16u) * 4u + r)));
     t.slab[r] = page * a.kv_heads + kv;
-    t.run[r] = uint64_t(t.slab[r]) * a.page_tokens + t.slot[r];
   }
   return t;
 }
@@ -239,6 +244,11 @@ __device__ __forceinline__ f16x8 as_f16x8(uint32_t a, uint32_t b, uint32_t c, ui
   return __builtin_bit_cast(f16x8, (u32x4_s{a, b, c, d}));
 }
 
+struct QPlace {
+  uint32_t block, kg, j;
+  bool odd;
+};
+
 // ---- cache formats: loads and operands of a tile, DIM = 32 G ------------------
 // token(kg, j): the tile's token of index j (0..7) of lane group kg.
 
@@ -259,11 +269,14 @@ struct Cache4 {
   static __device__ __forceinline__ uint32_t token(uint32_t kg, uint32_t j) { return 4u * j + kg; }
 
   // Lane's parameter words: token j = r / 2 of its group, blocks (r % 2) * G / 2 ..
-  static __device__ __forceinline__ Words<kPWords> params(const void* base, const TileRows& t, uint32_t r, uint32_t kg,
-                                                          uint32_t left) {
-    const uint32_t tok = token(kg, r / 2u);
-    const uint64_t row = pick(r / 4u, t.run[0], t.run[1], t.run[2], t.run[3]) + tok % 8u;
-    Words<kPWords> p = load_words<kPWords>(static_cast<const uint8_t*>(base) + row * (4u * G) + (r % 2u) * (2u * G));
+  template <bool ONE>
+  static __device__ __forceinline__ Words<kPWords> params(const void* base, const TileRows<ONE>& t, uint32_t P, uint32_t r,
+                                                          uint32_t kg, uint32_t left) {
+    const uint32_t tok = token(kg, r / 2u), in = (r % 2u) * (2u * G);
+    const uint8_t* b = static_cast<const uint8_t*>(base);
+    Words<kPWords> p;
+    if constexpr (ONE) p = load_words<kPWords>(b + t.row(0, P) * (4u * G) + (tok * (4u * G) + in));
+    else p = load_words<kPWords>(b + (pick(r / 4u, t.row(0, P), t.row(1, P), t.row(2, P), t.row(3, P)) + tok % 8u) * (4u * G) + in);
     if (tok >= left) {  // slots behind the sequence hold anything
 #pragma unroll
       for (int i = 0; i < kPWords; ++i) p.w[i] = 0u;
@@ -271,27 +284,39 @@ struct Cache4 {
     return p;
   }
   // A rows m: tokens 4 (m % 4) + m / 4 of the first 16, B those of the last 16.
-  static __device__ __forceinline__ K load_k(const ScoredArgs& a, const TileRows& t, uint32_t r, uint32_t kg,
+  template <bool ONE>
+  static __device__ __forceinline__ K load_k(const ScoredArgs& a, const TileRows<ONE>& t, uint32_t r, uint32_t kg,
                                              uint32_t left) {
-    const uint32_t in = (4u * (r % 4u) + r / 4u) % 8u;
-    const uint64_t ra = pick(r / 2u % 2u, t.run[0], t.run[1], 0ull, 0ull) + in, rb = pick(r / 2u % 2u, t.run[2], t.run[3], 0ull, 0ull) + in;
-    const uint8_t* base = static_cast<const uint8_t*>(a.k) + kg * (4u * G);
+    const uint32_t P = a.page_tokens, tok = 4u * (r % 4u) + r / 4u;
+    const uint8_t* base = static_cast<const uint8_t*>(a.k);
     K k;
-    k.a = load_words<G>(base + ra * (16u * G));
-    k.b = load_words<G>(base + rb * (16u * G));
-    k.p = params(a.ks, t, r, kg, left);
+    if constexpr (ONE) {
+      const uint8_t* first = base + t.row(0, P) * (16u * G);
+      const uint32_t at = tok * (16u * G) + kg * (4u * G);
+      k.a = load_words<G>(first + at);
+      k.b = load_words<G>(first + (at + 16u * (16u * G)));
+    } else {
+      const uint32_t in = (tok % 8u) * (16u * G) + kg * (4u * G);
+      const uint32_t second = r / 2u % 2u;
+      k.a = load_words<G>(base + pick<uint64_t>(second, t.row(0, P), t.row(1, P), 0u, 0u) * (16u * G) + in);
+      k.b = load_words<G>(base + pick<uint64_t>(second, t.row(2, P), t.row(3, P), 0u, 0u) * (16u * G) + in);
+    }
+    k.p = params<ONE>(a.ks, t, P, r, kg, left);
     return k;
   }
-  static __device__ __forceinline__ V load_v(const ScoredArgs& a, const TileRows& t, uint32_t r, uint32_t kg,
+  template <bool ONE>
+  static __device__ __forceinline__ V load_v(const ScoredArgs& a, const TileRows<ONE>& t, uint32_t r, uint32_t kg,
                                              uint32_t left) {
+    const uint32_t P = a.page_tokens, at = kg * (16u * G) + r * G;
     V v;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const uint8_t* p = static_cast<const uint8_t*>(a.v) + (t.run[j / 2] + 4u * (j % 2)) * (16u * G) + kg * (16u * G) + r * G;
+      const uint8_t* run = static_cast<const uint8_t*>(a.v) + t.row(ONE ? 0 : j / 2, P) * (16u * G);
+      const uint8_t* p = run + (at + 4u * uint32_t(ONE ? j : j % 2) * (16u * G));
       if constexpr (G == 2) v.v[j].w[0] = *reinterpret_cast<const uint16_t*>(p);
       else v.v[j] = load_words<kVWords>(p);
     }
-    v.p = params(a.vs, t, r, kg, left);
+    v.p = params<ONE>(a.vs, t, P, r, kg, left);
     return v;
   }
   // Eight codes of block g, dims 8 kg + (0, 2, 1, 3, 4, 6, 5, 7), the odd dims times 16.
@@ -311,12 +336,12 @@ struct Cache4 {
     }
     return as_f16x8(lo & 0x000f000fu, lo & 0x00f000f0u, hi & 0x000f000fu, hi & 0x00f000f0u);
   }
-  // Dim of Q element j of block g's operand, and whether its code is times 16.
-  static __device__ __forceinline__ uint32_t q_dim(int g, uint32_t kg, int j) {
-    constexpr uint32_t order[8] = {0, 2, 1, 3, 4, 6, 5, 7};
-    return 32u * g + 8u * kg + order[j];
+  // Where dim d stands in Q's operands: block, lane group, element; and whether
+  // its code is times 16.
+  static __device__ __forceinline__ QPlace q_place(uint32_t d) {
+    const uint32_t p = d % 8u;  // element order 0, 2, 1, 3, 4, 6, 5, 7
+    return QPlace{d / 32u, d / 8u % 4u, (p & 4u) | (p & 1u) << 1 | (p & 2u) >> 1, (p & 1u) != 0u};
   }
-  static constexpr bool q_odd(int j) { return (j & 2) != 0; }
 };
 
 template <int G>
@@ -334,107 +359,135 @@ struct Cache8 {
   };
   static __device__ __forceinline__ uint32_t token(uint32_t kg, uint32_t j) { return 8u * kg + j; }
   // Lanes r and r + 8: the scale of token r % 8 of the group.
-  static __device__ __forceinline__ float params(const float* base, const TileRows& t, uint32_t r, uint32_t kg,
-                                                 uint32_t left) {
-    const uint64_t row = pick(kg, t.run[0], t.run[1], t.run[2], t.run[3]);
-    const float p = base[row + r % 8u];
+  template <bool ONE>
+  static __device__ __forceinline__ float params(const void* base, const TileRows<ONE>& t, uint32_t P, uint32_t r,
+                                                 uint32_t kg, uint32_t left) {
+    const float* b = static_cast<const float*>(base);
+    const float p = ONE ? (b + t.row(0, P))[token(kg, r % 8u)]
+                        : b[pick(kg, t.row(0, P), t.row(1, P), t.row(2, P), t.row(3, P)) + r % 8u];
     return token(kg, r % 8u) < left ? p : 0.f;
   }
   // A rows m: tokens 8 (m / 4) + m % 4, B those four later.
-  static __device__ __forceinline__ K load_k(const ScoredArgs& a, const TileRows& t, uint32_t r, uint32_t kg,
+  template <bool ONE>
+  static __device__ __forceinline__ K load_k(const ScoredArgs& a, const TileRows<ONE>& t, uint32_t r, uint32_t kg,
                                              uint32_t left) {
-    const uint64_t run = pick(r / 4u, t.run[0], t.run[1], t.run[2], t.run[3]);
-    const uint8_t* base = static_cast<const uint8_t*>(a.k) + (run + r % 4u) * (32u * G) + kg * 16u;
+    const uint32_t P = a.page_tokens, D = 32u * G;
+    const uint8_t* base = static_cast<const uint8_t*>(a.k);
+    const uint8_t* first = ONE ? base + t.row(0, P) * D : base + pick(r / 4u, t.row(0, P), t.row(1, P), t.row(2, P), t.row(3, P)) * D;
+    const uint32_t at = (ONE ? 8u * (r / 4u) + r % 4u : r % 4u) * D + kg * 16u;
     K k;
 #pragma unroll
     for (int h = 0; h < G / 2; ++h) {  // 64 dims a piece: 16 bytes of each lane group
-      const Words<4> x = load_words<4>(base + 64u * h), y = load_words<4>(base + 64u * h + 4u * (32u * G));
+      const Words<4> x = load_words<4>(first + (at + 64u * h)), y = load_words<4>(first + (at + 64u * h + 4u * D));
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         k.a.w[4 * h + i] = x.w[i];
         k.b.w[4 * h + i] = y.w[i];
       }
     }
-    k.p = params(static_cast<const float*>(a.ks), t, r, kg, left);
+    k.p = params<ONE>(a.ks, t, P, r, kg, left);
     return k;
   }
   // Dim-major V: dim 16 f + r, the lane group's eight tokens.
-  static __device__ __forceinline__ V load_v(const ScoredArgs& a, const TileRows& t, uint32_t r, uint32_t kg,
+  template <bool ONE>
+  static __device__ __forceinline__ V load_v(const ScoredArgs& a, const TileRows<ONE>& t, uint32_t r, uint32_t kg,
                                              uint32_t left) {
-    const uint32_t slab = pick(kg, t.slab[0], t.slab[1], t.slab[2], t.slab[3]);
-    const uint32_t slot = pick(kg, t.slot[0], t.slot[1], t.slot[2], t.slot[3]);
-    const uint8_t* base = static_cast<const uint8_t*>(a.v) + uint64_t(slab) * (32u * G) * a.page_tokens + slot;
+    const uint32_t P = a.page_tokens, D = 32u * G;
+    const uint8_t* base = static_cast<const uint8_t*>(a.v);
     V v;
+    if constexpr (ONE) {
+      const uint8_t* slab = base + (uint64_t(t.slab[0]) * (uint64_t(D) * P) + t.slot[0]);
+      const uint64_t at = uint64_t(r) * P + 8u * kg;
 #pragma unroll
-    for (int f = 0; f < 2 * G; ++f) v.v[f] = load_words<2>(base + uint64_t(16u * f + r) * a.page_tokens);
-    v.p = params(static_cast<const float*>(a.vs), t, r, kg, left);
+      for (int f = 0; f < 2 * G; ++f) v.v[f] = load_words<2>(slab + uint64_t(16u * f) * P + at);
+    } else {
+      const uint32_t slab = pick(kg, t.slab[0], t.slab[1], t.slab[2], t.slab[3]);
+      const uint32_t slot = pick(kg, t.slot[0], t.slot[1], t.slot[2], t.slot[3]);
+      const uint8_t* first = base + uint64_t(slab) * (uint64_t(D) * P) + slot;
+#pragma unroll
+      for (int f = 0; f < 2 * G; ++f) v.v[f] = load_words<2>(first + uint64_t(16u * f + r) * P);
+    }
+    v.p = params<ONE>(a.vs, t, P, r, kg, left);
     return v;
   }
   template <int g>
   static __device__ __forceinline__ f16x8 k_frag(const Words<2 * G>& w) {
     return i8x8_to_f16(w.w[2 * g], w.w[2 * g + 1]);
   }
-  static __device__ __forceinline__ uint32_t q_dim(int g, uint32_t kg, int j) {
-    return 64u * (g / 2) + 16u * kg + 8u * (g % 2) + j;
+  static __device__ __forceinline__ QPlace q_place(uint32_t d) {
+    return QPlace{d / 64u * 2u + d / 8u % 2u, d / 16u % 4u, d % 8u, false};
   }
-  static constexpr bool q_odd(int) { return false; }
 };
 
 // ---- Q ---------------------------------------------------------------------------
-
-__device__ __forceinline__ float q_element(const void* q, uint64_t i, uint32_t type) {
-  if (type == 1u) return static_cast<const float*>(q)[i];
-  if (type == 2u) return float(static_cast<const _Float16*>(q)[i]);
-  return __uint_as_float(uint32_t(static_cast<const uint16_t*>(q)[i]) << 16);
-}
 
 // Digits of Q: two for 4 bits, and for fp32.
 template <class C, bool F32>
 constexpr int kQDigits = C::kBits == 4 || F32 ? 2 : 1;
 
-// One block's Q operands: fp16 digits of the scaled elements, the sums over
-// each 32 dims (4 bits, in units of 2^-24), and the score's factor.
+// The Q operands of a block of 16 head-rows in LDS, where every wave of the
+// work-group and every tile reads them: held in registers they took 32 (dim
+// 128) or 64 (dim 256) per lane and cost a third of the waves.
 template <class C, int QD>
 struct QBlock {
-  f16x8 d[C::kGroups][QD];
-  float sum[C::kBits == 4 ? C::kGroups : 1];
-  float factor;  // score = factor * (sum over dims of the scaled products)
+  f16x8 d[C::kGroups][QD][64];                     // fp16 digits of the scaled elements, by lane
+  float sum[C::kBits == 4 ? C::kGroups : 1][16];   // 4 bits: sum over each 32 dims, in units of 2^-24
+  float factor[16];                                // score = factor * (sum of the scaled products)
 };
 
+// By all 256 threads: thread 16 r + s takes 2 G dims from 2 G s of head-row r,
+// so that the maximum over a row is one over 16 lanes.  `at`: element index
+// of the head-row's Q.  The caller's barrier follows.
 template <class C, int QD>
-__device__ __forceinline__ QBlock<C, QD> load_q(const ScoredArgs& a, uint64_t at, bool valid, uint32_t kg) {
-  constexpr int G = C::kGroups;
-  QBlock<C, QD> q;
-  float x[G][8];
+__device__ __forceinline__ void stage_q(const ScoredArgs& a, uint64_t at, bool valid, QBlock<C, QD>& q) {
+  constexpr int G = C::kGroups, N = 2 * G;
+  const uint32_t r = threadIdx.x / 16u, s = threadIdx.x % 16u, d0 = s * N;
+  float x[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) x[i] = 0.f;
+  if (valid) {
+    if (a.q_type == 1u) {
+      const float* p = static_cast<const float*>(a.q) + at + d0;
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[i] = p[i];
+    } else {
+      const uint16_t* p = static_cast<const uint16_t*>(a.q) + at + d0;
+      uint16_t u[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) u[i] = p[i];
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        x[i] = a.q_type == 2u ? float(__builtin_bit_cast(_Float16, u[i])) : __uint_as_float(uint32_t(u[i]) << 16);
+    }
+  }
   float top = 0.f;
 #pragma unroll
-  for (int g = 0; g < G; ++g)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      x[g][j] = valid ? q_element(a.q, at + C::q_dim(g, kg, j), a.q_type) : 0.f;
-      top = fmaxf(top, fabsf(x[g][j]));
-    }
-  top = rows_max(top);
+  for (int i = 0; i < N; ++i) top = fmaxf(top, fabsf(x[i]));
+  top = fmaxf(top, row_ror<8>(top));
+  top = fmaxf(top, row_ror<4>(top));
+  top = fmaxf(top, row_ror<2>(top));
+  top = fmaxf(top, row_ror<1>(top));
   int up = 0;  // an infinite or NaN element: the row's result is NaN whatever the scale
   if (top > 0.f && top <= FLT_MAX) up = 14 - __builtin_amdgcn_frexp_expf(top);  // frexp: top = f * 2^e, f in [1/2, 1)
-  q.factor = ldexpf(a.scale, (C::kBits == 4 ? 24 : 0) - up);
+  float sum = 0.f;
 #pragma unroll
-  for (int g = 0; g < G; ++g) {
-    float s = 0.f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      float y = ldexpf(x[g][j], up);
-      s += y;
-      if (C::q_odd(j)) y *= 0.0625f;
-      // 4 bits: multiples of 8 up to 2^14 (odd dims: both a 16th)
-      const float unit = C::q_odd(j) ? 0.5f : 8.f;
-      const _Float16 hi = C::kBits == 4 ? _Float16(__builtin_rintf(y * (1.f / unit)) * unit) : _Float16(y);
-      q.d[g][0][j] = hi;
-      if constexpr (QD == 2) q.d[g][1][j] = _Float16(y - float(hi));
-    }
-    if constexpr (C::kBits == 4) q.sum[g] = ldexpf(rows_sum(s), -24);
+  for (int i = 0; i < N; ++i) {
+    const QPlace p = C::q_place(d0 + i);
+    float y = ldexpf(x[i], up);
+    sum += y;
+    if (p.odd) y *= 0.0625f;
+    // 4 bits: multiples of 8 up to 2^14 (odd dims: both a 16th)
+    const float unit = p.odd ? 0.5f : 8.f, per = p.odd ? 2.f : 0.125f;
+    const _Float16 hi = C::kBits == 4 ? _Float16(__builtin_rintf(y * per) * unit) : _Float16(y);
+    reinterpret_cast<_Float16*>(&q.d[p.block][0][p.kg * 16u + r])[p.j] = hi;
+    if constexpr (QD == 2) reinterpret_cast<_Float16*>(&q.d[p.block][1][p.kg * 16u + r])[p.j] = _Float16(y - float(hi));
   }
-  return q;
+  if constexpr (C::kBits == 4) {  // 16 / G threads hold a block's 32 dims
+#pragma unroll
+    for (int o = 1; o < 16 / G; o <<= 1) sum += __shfl_xor(sum, o);
+    if (s % (16u / G) == 0u) q.sum[s / (16u / G)][r] = ldexpf(sum, -24);
+  }
+  if (s == 0u) q.factor[r] = ldexpf(a.scale, (C::kBits == 4 ? 24 : 0) - up);
 }
 
 // ---- scores ------------------------------------------------------------------------
@@ -442,7 +495,7 @@ __device__ __forceinline__ QBlock<C, QD> load_q(const ScoredArgs& a, uint64_t at
 // The products of a tile: x[j] = sum of step / scale times products plus least
 // value times Q sums, before the score's factor.
 template <class C, int QD>
-__device__ __forceinline__ void tile_scores(const typename C::K& k, const QBlock<C, QD>& q, float (&x)[8]) {
+__device__ __forceinline__ void tile_scores(const typename C::K& k, const QBlock<C, QD>& q, uint32_t lane, float (&x)[8]) {
   constexpr int G = C::kGroups;
   const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
   if constexpr (C::kBits == 4) {
@@ -458,17 +511,19 @@ __device__ __forceinline__ void tile_scores(const typename C::K& k, const QBlock
     unrolled<0, G>([&](auto gc) {
       constexpr int g = gc;
       const f16x8 ka = C::template k_frag<g>(k.a), kb = C::template k_frag<g>(k.b);
-      f32x4 da = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, q.d[g][0], zero, 0, 0, 0);
-      f32x4 db = __builtin_amdgcn_mfma_f32_16x16x32_f16(kb, q.d[g][0], zero, 0, 0, 0);
-      if constexpr (QD == 2) {
-        da = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, q.d[g][1], da, 0, 0, 0);
-        db = __builtin_amdgcn_mfma_f32_16x16x32_f16(kb, q.d[g][1], db, 0, 0, 0);
+      f32x4 da = zero, db = zero;
+#pragma unroll
+      for (int i = 0; i < QD; ++i) {
+        const f16x8 qd = q.d[g][i][lane];
+        da = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qd, da, 0, 0, 0);
+        db = __builtin_amdgcn_mfma_f32_16x16x32_f16(kb, qd, db, 0, 0, 0);
       }
+      const float sum = q.sum[g][lane % 16u];
       unrolled<0, 8>([&](auto jc) {
-        constexpr int j = jc, lane = 2 * j + g / PW, i = g % PW;
+        constexpr int j = jc, from = 2 * j + g / PW, i = g % PW;
         const float d = j < 4 ? da[j % 4] : db[j % 4];
-        x[j] = fmaf(bc<lane>(st[i]), d, x[j]);
-        x[j] = fmaf(bc<lane>(le[i]), q.sum[g], x[j]);
+        x[j] = fmaf(bc<from>(st[i]), d, x[j]);
+        x[j] = fmaf(bc<from>(le[i]), sum, x[j]);
       });
     });
   } else {
@@ -478,8 +533,9 @@ __device__ __forceinline__ void tile_scores(const typename C::K& k, const QBlock
       const f16x8 ka = C::template k_frag<g>(k.a), kb = C::template k_frag<g>(k.b);
 #pragma unroll
       for (int i = 0; i < QD; ++i) {
-        da = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, q.d[g][i], da, 0, 0, 0);
-        db = __builtin_amdgcn_mfma_f32_16x16x32_f16(kb, q.d[g][i], db, 0, 0, 0);
+        const f16x8 qd = q.d[g][i][lane];
+        da = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qd, da, 0, 0, 0);
+        db = __builtin_amdgcn_mfma_f32_16x16x32_f16(kb, qd, db, 0, 0, 0);
       }
     });
     unrolled<0, 8>([&](auto jc) {
@@ -507,7 +563,7 @@ __device__ __forceinline__ int near(int64_t d) {
 }
 
 // Score forms on a tile's products: factor, cap, bias by distance, and -inf
-// where MASKED and not visible.  Scores stay in natural units: their difference
+// where the tile is masked and the token not visible.  Scores stay in natural units: their difference
 // to a reference is taken first and then multiplied by log2(e) for the
 // exponential.  With the two constants in one rounded factor instead, l of 512
 // tokens was off by 1.1e-6, since every score carried the same relative error.
@@ -518,9 +574,9 @@ struct ScoreForm {
 __device__ __forceinline__ ScoreForm score_form(const ScoredArgs& a, float factor, float slope, int back) {
   return ScoreForm{factor, a.cap, a.cap > 0.f ? 1.f / a.cap : 0.f, slope, back};
 }
-template <class C, bool MASKED>
+template <class C>
 __device__ __forceinline__ void apply_form(const ScoredArgs& a, const ScoreForm& f, int ahead, uint32_t t0, uint32_t kg,
-                                           const Visible& v, float (&x)[8]) {
+                                           bool masked, uint32_t lo, uint32_t hi, uint32_t pre, float (&x)[8]) {
 #pragma unroll
   for (int j = 0; j < 8; ++j) x[j] *= f.factor;
   if (a.cap > 0.f) {
@@ -533,11 +589,11 @@ __device__ __forceinline__ void apply_form(const ScoredArgs& a, const ScoreForm&
       x[j] = fmaf(f.slope, float(bci<j>(ahead) - f.back), x[j]);
     });
   }
-  if constexpr (MASKED) {
+  if (masked) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const uint32_t t = t0 + C::token(kg, j);
-      const bool seen = (t >= v.lo && t < v.hi) || t < v.pre;
+      const bool seen = (t >= lo && t < hi) || t < pre;
       x[j] = seen ? x[j] : neg_inf();
     }
   }

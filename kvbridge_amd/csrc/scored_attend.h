@@ -111,33 +111,74 @@ __device__ __forceinline__ PDigits<PD> p_digits(const float (&w)[8]) {
   return p;
 }
 
-// One tile's weights and their products with V.  MASKED: some head-row does
-// not see every token, whose parameters may be anything.
-template <int G, int PD, bool MASKED>
-__device__ __forceinline__ void tile_values(const ScoredArgs&, const typename Cache4<G>::V& v, const float (&x)[8],
-                                            AttendState<Cache4<G>>& s, uint32_t) {
-  using C = Cache4<G>;
-  constexpr int PW = C::kPWords;
+// Whether a tile asks for another reference or scale: p < 2^8 and step * 2^ve
+// <= 2^7 keep every weight below 2^16.  And the rescale itself.
+template <int G>
+__device__ __forceinline__ void keep_range(const typename Cache4<G>::V& v, const float (&x)[8], AttendState<Cache4<G>>& s) {
+  constexpr int PW = Cache4<G>::kPWords;
+  float st[PW], top = 0.f;
+#pragma unroll
+  for (int i = 0; i < PW; ++i) {
+    st[i] = __uint_as_float(v.p.w[i] & 0xffff0000u);
+    top = fmaxf(top, st[i]);
+  }
+  if (!__any(s.mtop > s.mref + 5.5f || top * s.vf > 128.f)) return;
+  rescale(s, x, [&](auto jc) {
+    constexpr int j = jc;
+    float t = 0.f;
+    unrolled<0, G>([&](auto gc) {
+      constexpr int g = gc, lane = 2 * j + g / PW, i = g % PW;
+      t = fmaxf(t, bc<lane>(st[i]));
+    });
+    return t;
+  });
+}
+template <int G>
+__device__ __forceinline__ void keep_range(const typename Cache8<G>::V& v, const float (&x)[8], AttendState<Cache8<G>>& s) {
+  if (!__any(s.mtop > s.mref + 5.5f || v.p * s.vf > 128.f)) return;
+  rescale(s, x, [&](auto jc) {
+    constexpr int j = jc;
+    return bc<j>(v.p);
+  });
+}
+
+// A tile in which some head-row does not see every token: an infinite or NaN
+// parameter times the weight 0 would reach that head-row.  Such parameters
+// become 0, and the head-rows that do see the token get a NaN in its block.
+template <int G>
+__device__ __forceinline__ void hide_odd_params(typename Cache4<G>::V& v, const float (&x)[8], AttendState<Cache4<G>>& s,
+                                                uint32_t kg) {
+  constexpr int PW = Cache4<G>::kPWords;
+  bool odd[PW], any = false;
+#pragma unroll
+  for (int i = 0; i < PW; ++i) {
+    odd[i] = (v.p.w[i] & 0x7f800000u) == 0x7f800000u || (v.p.w[i] & 0x7f80u) == 0x7f80u;
+    any = any || odd[i];
+  }
+  if (!__any(any)) return;
+  uint32_t seen = 0u;  // bit 2 j: the lane's token j has a weight
+#pragma unroll
+  for (int j = 0; j < 8; ++j) seen |= exp_e(x[j] - s.mref) != 0.f ? 1u << (2 * j) : 0u;
+#pragma unroll
+  for (int i = 0; i < PW; ++i) {
+    const uint32_t lanes = uint32_t(__ballot(odd[i]) >> (16u * kg));  // bit 2 j + h: token j, block h * PW + i
+    s.mid[i] = (lanes & seen) != 0u ? __builtin_nanf("") : s.mid[i];
+    s.mid[PW + i] = ((lanes >> 1) & seen) != 0u ? __builtin_nanf("") : s.mid[PW + i];
+    v.p.w[i] = odd[i] ? 0u : v.p.w[i];
+  }
+}
+template <int G>
+__device__ __forceinline__ void hide_odd_params(typename Cache8<G>::V&, const float (&)[8], AttendState<Cache8<G>>&, uint32_t) {}
+
+// One tile's weights and their products with V.
+template <int G, int PD>
+__device__ __forceinline__ void tile_values(const typename Cache4<G>::V& v, const float (&x)[8], AttendState<Cache4<G>>& s) {
+  constexpr int PW = Cache4<G>::kPWords;
   float st[PW], mid[PW];
 #pragma unroll
   for (int i = 0; i < PW; ++i) {
     st[i] = __uint_as_float(v.p.w[i] & 0xffff0000u);
     mid[i] = fmaf(st[i], 8.f, __uint_as_float(v.p.w[i] << 16));
-  }
-  float top = 0.f;
-#pragma unroll
-  for (int i = 0; i < PW; ++i) top = fmaxf(top, st[i]);
-  // p < 2^8 and step * 2^ve < 2^7: no weight reaches 2^16
-  if (__any(s.mtop > s.mref + 5.5f) || __any(top * s.vf > 128.f)) {
-    rescale(s, x, [&](auto jc) {
-      constexpr int j = jc;
-      float t = 0.f;
-      unrolled<0, G>([&](auto gc) {
-        constexpr int g = gc, lane = 2 * j + g / PW, i = g % PW;
-        t = fmaxf(t, bc<lane>(st[i]));
-      });
-      return t;
-    });
   }
   float p[8], pv[8];
 #pragma unroll
@@ -152,14 +193,8 @@ __device__ __forceinline__ void tile_values(const ScoredArgs&, const typename Ca
     unrolled<0, 8>([&](auto jc) {
       constexpr int j = jc, lane = 2 * j + g / PW, i = g % PW;
       const float step = bc<lane>(st[i]), at8 = bc<lane>(mid[i]);
-      if constexpr (MASKED) {
-        const bool in = p[j] != 0.f;
-        w[j] = in ? step * pv[j] : 0.f;
-        s.mid[g] = in ? fmaf(at8, p[j], s.mid[g]) : s.mid[g];
-      } else {
-        w[j] = step * pv[j];
-        s.mid[g] = fmaf(at8, p[j], s.mid[g]);
-      }
+      w[j] = step * pv[j];
+      s.mid[g] = fmaf(at8, p[j], s.mid[g]);
     });
     const PDigits<PD> d = p_digits<PD>(w);
     uint32_t u[4];
@@ -180,23 +215,17 @@ __device__ __forceinline__ void tile_values(const ScoredArgs&, const typename Ca
       s.acc[2 * g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, d.d[i], s.acc[2 * g], 0, 0, 0);
       s.acc[2 * g + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, d.d[i], s.acc[2 * g + 1], 0, 0, 0);
     }
+    __builtin_amdgcn_sched_barrier(0);  // one block's operands at a time in registers
   });
 }
-template <int G, int PD, bool MASKED>
-__device__ __forceinline__ void tile_values(const ScoredArgs&, const typename Cache8<G>::V& v, const float (&x)[8],
-                                            AttendState<Cache8<G>>& s, uint32_t) {
-  if (__any(s.mtop > s.mref + 5.5f) || __any(v.p * s.vf > 128.f)) {
-    rescale(s, x, [&](auto jc) {
-      constexpr int j = jc;
-      return bc<j>(v.p);
-    });
-  }
+template <int G, int PD>
+__device__ __forceinline__ void tile_values(const typename Cache8<G>::V& v, const float (&x)[8], AttendState<Cache8<G>>& s) {
   float p[8], w[8];
   unrolled<0, 8>([&](auto jc) {
     constexpr int j = jc;
     p[j] = exp_e(x[j] - s.mref);
     w[j] = bc<j>(v.p) * (p[j] * s.vf);
-    if (MASKED && p[j] == 0.f) w[j] = 0.f;
+    w[j] = p[j] == 0.f ? 0.f : w[j];
   });
   s.l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
   const PDigits<PD> d = p_digits<PD>(w);
@@ -223,14 +252,22 @@ __device__ __forceinline__ f32x4 chunk_value(const AttendState<Cache8<G>>& s, in
   return f32x4{s.acc[c][0] * f, s.acc[c][1] * f, s.acc[c][2] * f, s.acc[c][3] * f};
 }
 template <class C>
-__device__ __forceinline__ uint32_t chunk_dim(int c, uint32_t kg) {
-  return C::kBits == 4 ? 32u * (c / 2) + 8u * kg + 4u * (c % 2) : 16u * c + 4u * kg;
+__device__ __forceinline__ uint32_t chunk_dim(uint32_t c, uint32_t kg) {
+  return C::kBits == 4 ? 32u * (c / 2u) + 8u * kg + 4u * (c % 2u) : 16u * c + 4u * kg;
 }
 
-template <class C, int QD, int PD>
-__global__ __launch_bounds__(64 * kAttendWaves) void scored_attend_kernel(const ScoredArgs a) {
-  constexpr int G = C::kGroups, NC = 2 * G, NW = kAttendWaves;
-  __shared__ f32x4 lds_o[NW][NC][64];
+// LDS: Q's operands while the tiles run, then the waves' numerators, eight
+// chunks at a time (all of dim 64 and 128, half of dim 256).
+template <class C, int QD>
+union AttendLds {
+  QBlock<C, QD> q;
+  f32x4 o[kAttendWaves][2 * C::kGroups < 8 ? 2 * C::kGroups : 8][64];
+};
+
+template <class C, int QD, int PD, bool ONE>
+__global__ __launch_bounds__(64 * kAttendWaves, C::kGroups == 8 ? 2 : 3) void scored_attend_kernel(const ScoredArgs a) {
+  constexpr int G = C::kGroups, NC = 2 * G, NW = kAttendWaves, NR = NC < 8 ? NC : 8;
+  __shared__ AttendLds<C, QD> lds;
   __shared__ float lds_m[NW][16], lds_l[NW][16];
   const uint32_t lane = threadIdx.x & 63u, r = lane & 15u, kg = lane >> 4;
   const uint32_t wave = uint32_t(__builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6)));
@@ -262,10 +299,14 @@ __global__ __launch_bounds__(64 * kAttendWaves) void scored_attend_kernel(const 
     }
     return;
   }
-
-  const uint64_t q_at = (uint64_t(b) * a.rows + row) * a.q_stride + uint64_t(head) * a.dim;
-  const QBlock<C, QD> q = load_q<C, QD>(a, q_at, valid, kg);
-  const ScoreForm form = score_form(a, q.factor, a.slopes ? a.slopes[head] : 0.f, near(int64_t(uint64_t(qpos) - uint64_t(qref))));
+  {
+    const uint32_t q_hr = block * 16u + threadIdx.x / 16u;
+    const uint32_t q_row = q_hr / a.group;
+    stage_q<C, QD>(a, (uint64_t(b) * a.rows + q_row) * a.q_stride + uint64_t(kv * a.group + q_hr % a.group) * a.dim,
+                   q_hr < a.head_rows, lds.q);
+  }
+  __syncthreads();
+  const ScoreForm form = score_form(a, lds.q.factor[r], a.slopes ? a.slopes[head] : 0.f, near(int64_t(uint64_t(qpos) - uint64_t(qref))));
 
   AttendState<C> s;
 #pragma unroll
@@ -287,33 +328,27 @@ __global__ __launch_bounds__(64 * kAttendWaves) void scored_attend_kernel(const 
   };
   if (n > 0u) {
     TilePages pages = tile_pages(a, e, tile_of, 0u, lane), ahead_pages = pages;
-    TileRows rows = tile_rows(a, pages, 0u, kv);
+    TileRows<ONE> rows = tile_rows<ONE>(a, pages, 0u, kv);
     uint32_t t0 = tile_of(0u) * kTileTokens;
-    typename C::K k = C::load_k(a, rows, r, kg, e.tokens - t0);
+    typename C::K k = C::template load_k<ONE>(a, rows, r, kg, e.tokens - t0);
     int ahead = load_ahead<C>(a, e, t0, r, kg, qref);
     for (uint32_t i = 0; i < n; ++i) {
       if (i % 16u == 0u) ahead_pages = tile_pages(a, e, tile_of, i + 16u, lane);  // a window ahead
-      const typename C::V v = C::load_v(a, rows, r, kg, e.tokens - t0);
+      typename C::V v = C::template load_v<ONE>(a, rows, r, kg, e.tokens - t0);
       const uint32_t t_next = tile_of(i + 1u < n ? i + 1u : i) * kTileTokens;
       if ((i + 1u) % 16u == 0u) pages = ahead_pages;
-      const TileRows rows_next = tile_rows(a, pages, i + 1u < n ? i + 1u : i, kv);
-      const typename C::K k_next = C::load_k(a, rows_next, r, kg, e.tokens - t_next);
+      const TileRows<ONE> rows_next = tile_rows<ONE>(a, pages, i + 1u < n ? i + 1u : i, kv);
+      const typename C::K k_next = C::template load_k<ONE>(a, rows_next, r, kg, e.tokens - t_next);
       const int ahead_next = load_ahead<C>(a, e, t_next, r, kg, qref);
+      asm volatile("" ::: "memory");  // Q's operands stay in LDS: not hoisted out of the loop
       float x[8];
-      tile_scores<C, QD>(k, q, x);
+      tile_scores<C, QD>(k, lds.q, lane, x);
       const bool whole = t0 + kTileTokens <= vis.pre || (t0 >= vis.all_lo && t0 + kTileTokens <= vis.all_hi);
-      const auto tops = [&] {
-        s.mtop = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])), s.mtop));
-      };
-      if (whole) {
-        apply_form<C, false>(a, form, ahead, t0, kg, vis, x);
-        tops();
-        tile_values<G, PD, false>(a, v, x, s, kg);
-      } else {
-        apply_form<C, true>(a, form, ahead, t0, kg, vis, x);
-        tops();
-        tile_values<G, PD, true>(a, v, x, s, kg);
-      }
+      apply_form<C>(a, form, ahead, t0, kg, !whole, vis.lo, vis.hi, vis.pre, x);
+      s.mtop = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])), s.mtop));
+      keep_range<G>(v, x, s);
+      if (!whole) hide_odd_params<G>(v, x, s, kg);
+      tile_values<G, PD>(v, x, s);
       k = k_next;
       rows = rows_next;
       t0 = t_next;
@@ -327,41 +362,47 @@ __global__ __launch_bounds__(64 * kAttendWaves) void scored_attend_kernel(const 
   float mid[C::kBits == 4 ? G : 1];
 #pragma unroll
   for (int g = 0; g < (C::kBits == 4 ? G : 1); ++g) mid[g] = rows_sum(s.mid[g]);
-  __syncthreads();
+  __syncthreads();  // also: every wave is done with Q
   float top = lds_m[0][r];
 #pragma unroll
   for (int w = 1; w < NW; ++w) top = fmaxf(top, lds_m[w][r]);
   // A wave without visible tokens has mref = -FLT_MAX: a factor of 0.
   const float f = l == 0.f ? 0.f : exp_e(s.mref - top);
-#pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    f32x4 o = chunk_value(s, c, mid);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = l == 0.f ? 0.f : o[i] * f;
-    lds_o[wave][c][lane] = o;
-  }
   if (kg == 0u) lds_l[wave][r] = l * f;
-  __syncthreads();
-  float sum = lds_l[0][r];
-#pragma unroll
-  for (int w = 1; w < NW; ++w) sum += lds_l[w][r];
   const bool done = own == 1u;
   const PartialPlace part = done ? PartialPlace{nullptr, nullptr} : partial_place(a, rh, split);
+  float sum = 0.f;
 #pragma unroll
-  for (int i = 0; i < NC / NW; ++i) {
-    const int c = wave * (NC / NW) + i;
-    f32x4 o = lds_o[0][c][lane];
+  for (int round = 0; round < NC / NR; ++round) {
 #pragma unroll
-    for (int w = 1; w < NW; ++w) o += lds_o[w][c][lane];
-    if (!valid) continue;
-    const uint32_t d = chunk_dim<C>(c, kg);
-    if (done) {
+    for (int c = 0; c < NR; ++c) {
+      f32x4 o = chunk_value(s, round * NR + c, mid);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) o[k] = sum == 0.f ? 0.f : o[k] / sum;
-      store_out4(a, rh * a.dim + d, o);
-    } else {
-      *reinterpret_cast<f32x4*>(part.o + d) = o;
+      for (int i = 0; i < 4; ++i) o[i] = l == 0.f ? 0.f : o[i] * f;
+      lds.o[wave][c][lane] = o;
     }
+    __syncthreads();
+    if (round == 0) {
+#pragma unroll
+      for (int w = 0; w < NW; ++w) sum += lds_l[w][r];
+    }
+#pragma unroll
+    for (int i = 0; i < NR / NW; ++i) {
+      const uint32_t c = wave * (NR / NW) + i;
+      f32x4 o = lds.o[0][c][lane];
+#pragma unroll
+      for (int w = 1; w < NW; ++w) o += lds.o[w][c][lane];
+      if (!valid) continue;
+      const uint32_t d = chunk_dim<C>(round * NR + c, kg);
+      if (done) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[k] = sum == 0.f ? 0.f : o[k] / sum;
+        store_out4(a, rh * a.dim + d, o);
+      } else {
+        *reinterpret_cast<f32x4*>(part.o + d) = o;
+      }
+    }
+    if (round + 1 < NC / NR) __syncthreads();
   }
   if (wave == 0u && valid && kg == 0u) {
     if (done) {
@@ -419,7 +460,8 @@ __global__ __launch_bounds__(256) void scored_merge_kernel(const ScoredArgs a) {
 template <class C, int QD, int PD>
 inline hipError_t launch_attend_kernel(const ScoredArgs& a, hipStream_t stream) {
   const uint32_t groups = a.batch * a.splits * a.blocks * a.kv_heads;
-  scored_attend_kernel<C, QD, PD><<<groups, 64 * kAttendWaves, 0, stream>>>(a);
+  if (a.page_tokens % kTileTokens == 0u) scored_attend_kernel<C, QD, PD, true><<<groups, 64 * kAttendWaves, 0, stream>>>(a);
+  else scored_attend_kernel<C, QD, PD, false><<<groups, 64 * kAttendWaves, 0, stream>>>(a);
   return hipGetLastError();
 }
 // Weights of one digit only where the output is bf16 and q has 16 bits.
