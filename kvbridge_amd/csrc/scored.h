@@ -24,8 +24,16 @@
 // 4 bits, V: the same cancellation over a whole context would cost 2e-5 of an
 // output, so codes enter as c - 8 (one v_and_or_b32 and half a v_pk_add_f16 more
 // per two codes) and the block's value at code 8 replaces the least.
-// The block parameters of a lane's tokens lie in the 16 lanes of its row and are
-// read by DPP row broadcasts inside the multiply-adds.
+// With few head-rows most of the 16 columns would be idle while every lane
+// multiplies all G parameters of its tokens.  Instead column r * F + f holds
+// head-row r's Q of the blocks f * H .. f * H + H - 1 (G = F H) and zeros
+// elsewhere: the products of all blocks then accumulate in H results, a lane
+// applies the parameters of its H blocks only (loaded by itself), and a sum over
+// F neighbouring lanes makes the score; likewise the weights times the steps
+// and the values at code 8.  That was 592 -> 350 vector instructions per tile
+// at dim 128 and four head-rows (F = 4).  F = 1 (more head-rows than 16 / F):
+// the parameters of a lane's tokens lie in the 16 lanes of its row and are read
+// by DPP row broadcasts.
 // 8 bits: codes are converted exactly (i8x8_to_f16), the per-token scale
 // multiplies the sum.
 //
@@ -249,15 +257,28 @@ struct QPlace {
   bool odd;
 };
 
+// Sum over the F lanes of a head-row, in every one of them.
+template <int F>
+__device__ __forceinline__ float lanes_sum(float x) {
+  if constexpr (F >= 2) x += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0xB1, 0xF, 0xF, true));   // lane ^ 1
+  if constexpr (F >= 4) x += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x4E, 0xF, 0xF, true));   // lane ^ 2
+  if constexpr (F >= 8) x += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x141, 0xF, 0xF, true));  // lane 7 - l of 8
+  return x;
+}
+
 // ---- cache formats: loads and operands of a tile, DIM = 32 G ------------------
 // token(kg, j): the tile's token of index j (0..7) of lane group kg.
 
-template <int G>
+template <int G, int F>
 struct Cache4 {
   static constexpr int kGroups = G;
+  static constexpr int kF = F;
+  static constexpr int kH = G / F;  // blocks of a lane
   static constexpr int kBits = 4;
   static constexpr int kVWords = G >= 4 ? G / 4 : 1;
-  static constexpr int kPWords = G / 2;  // parameter words of a lane: word w of a lane group lies in lane w / kPWords
+  // Parameter words of a lane.  F = 1: word w of a lane group's 8 G lies in lane
+  // w / kPWords; else the lane's own blocks of its eight tokens.
+  static constexpr int kPWords = F == 1 ? G / 2 : 8 * kH;
   struct K {
     Words<G> a, b;
     Words<kPWords> p;
@@ -268,18 +289,60 @@ struct Cache4 {
   };
   static __device__ __forceinline__ uint32_t token(uint32_t kg, uint32_t j) { return 4u * j + kg; }
 
-  // Lane's parameter words: token j = r / 2 of its group, blocks (r % 2) * G / 2 ..
   template <bool ONE>
   static __device__ __forceinline__ Words<kPWords> params(const void* base, const TileRows<ONE>& t, uint32_t P, uint32_t r,
                                                           uint32_t kg, uint32_t left) {
-    const uint32_t tok = token(kg, r / 2u), in = (r % 2u) * (2u * G);
     const uint8_t* b = static_cast<const uint8_t*>(base);
     Words<kPWords> p;
-    if constexpr (ONE) p = load_words<kPWords>(b + t.row(0, P) * (4u * G) + (tok * (4u * G) + in));
-    else p = load_words<kPWords>(b + (pick(r / 4u, t.row(0, P), t.row(1, P), t.row(2, P), t.row(3, P)) + tok % 8u) * (4u * G) + in);
-    if (tok >= left) {  // slots behind the sequence hold anything
+    if constexpr (F == 1) {  // token j = r / 2 of the lane group, blocks (r % 2) * G / 2 ..
+      const uint32_t tok = token(kg, r / 2u), in = (r % 2u) * (2u * G);
+      if constexpr (ONE) p = load_words<kPWords>(b + t.row(0, P) * (4u * G) + (tok * (4u * G) + in));
+      else p = load_words<kPWords>(b + (pick(r / 4u, t.row(0, P), t.row(1, P), t.row(2, P), t.row(3, P)) + tok % 8u) * (4u * G) + in);
+      if (tok >= left) {  // slots behind the sequence hold anything
 #pragma unroll
-      for (int i = 0; i < kPWords; ++i) p.w[i] = 0u;
+        for (int i = 0; i < kPWords; ++i) p.w[i] = 0u;
+      }
+    } else {
+      const uint32_t at = kg * (4u * G) + r % F * (4u * kH);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint8_t* run = b + t.row(ONE ? 0 : j / 2, P) * (4u * G);
+        const Words<kH> w = load_words<kH>(run + (at + 4u * uint32_t(ONE ? j : j % 2) * (4u * G)));
+#pragma unroll
+        for (int h = 0; h < kH; ++h) p.w[j * kH + h] = w.w[h];
+      }
+      if (left < kTileTokens) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+          for (int h = 0; h < kH; ++h) p.w[j * kH + h] = token(kg, j) < left ? p.w[j * kH + h] : 0u;
+      }
+    }
+    return p;
+  }
+  // The parameters as floats, and those of token j and the lane's block h.
+  struct Params {
+    float step[kPWords], other[kPWords];
+    template <int j, int h>
+    __device__ __forceinline__ float step_of() const {
+      if constexpr (F == 1) return bc<2 * j + h / kPWords>(step[h % kPWords]);
+      else return step[j * kH + h];
+    }
+    template <int j, int h>
+    __device__ __forceinline__ float other_of() const {
+      if constexpr (F == 1) return bc<2 * j + h / kPWords>(other[h % kPWords]);
+      else return other[j * kH + h];
+    }
+  };
+  // AT8: the value at code 8 in place of the least.
+  template <bool AT8>
+  static __device__ __forceinline__ Params unpack(const Words<kPWords>& w) {
+    Params p;
+#pragma unroll
+    for (int i = 0; i < kPWords; ++i) {
+      p.step[i] = __uint_as_float(w.w[i] & 0xffff0000u);
+      p.other[i] = __uint_as_float(w.w[i] << 16);
+      if constexpr (AT8) p.other[i] = fmaf(p.step[i], 8.f, p.other[i]);
     }
     return p;
   }
@@ -347,6 +410,7 @@ struct Cache4 {
 template <int G>
 struct Cache8 {
   static constexpr int kGroups = G;
+  static constexpr int kF = 1, kH = G;
   static constexpr int kBits = 8;
   static constexpr int kPWords = 1;
   struct K {
@@ -431,7 +495,7 @@ constexpr int kQDigits = C::kBits == 4 || F32 ? 2 : 1;
 template <class C, int QD>
 struct QBlock {
   f16x8 d[C::kGroups][QD][64];                     // fp16 digits of the scaled elements, by lane
-  float sum[C::kBits == 4 ? C::kGroups : 1][16];   // 4 bits: sum over each 32 dims, in units of 2^-24
+  float sum[C::kBits == 4 ? C::kH : 1][16];        // 4 bits: sum over each 32 dims, in units of 2^-24, by column
   float factor[16];                                // score = factor * (sum of the scaled products)
 };
 
@@ -441,7 +505,16 @@ struct QBlock {
 template <class C, int QD>
 __device__ __forceinline__ void stage_q(const ScoredArgs& a, uint64_t at, bool valid, QBlock<C, QD>& q) {
   constexpr int G = C::kGroups, N = 2 * G;
+  constexpr int F = C::kF, H = C::kH;
   const uint32_t r = threadIdx.x / 16u, s = threadIdx.x % 16u, d0 = s * N;
+  if constexpr (F > 1) {
+    const f16x8 zero = {0, 0, 0, 0, 0, 0, 0, 0};
+    f16x8* all = &q.d[0][0][0];
+#pragma unroll
+    for (int i = 0; i < G * QD / 4; ++i) all[i * 256 + threadIdx.x] = zero;
+    __syncthreads();
+    if (r >= 16u / F) return;
+  }
   float x[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) x[i] = 0.f;
@@ -479,15 +552,18 @@ __device__ __forceinline__ void stage_q(const ScoredArgs& a, uint64_t at, bool v
     // 4 bits: multiples of 8 up to 2^14 (odd dims: both a 16th)
     const float unit = p.odd ? 0.5f : 8.f, per = p.odd ? 2.f : 0.125f;
     const _Float16 hi = C::kBits == 4 ? _Float16(__builtin_rintf(y * per) * unit) : _Float16(y);
-    reinterpret_cast<_Float16*>(&q.d[p.block][0][p.kg * 16u + r])[p.j] = hi;
-    if constexpr (QD == 2) reinterpret_cast<_Float16*>(&q.d[p.block][1][p.kg * 16u + r])[p.j] = _Float16(y - float(hi));
+    const uint32_t column = r * F + p.block / H;
+    reinterpret_cast<_Float16*>(&q.d[p.block][0][p.kg * 16u + (F > 1 ? column : r)])[p.j] = hi;
+    if constexpr (QD == 2)
+      reinterpret_cast<_Float16*>(&q.d[p.block][1][p.kg * 16u + (F > 1 ? column : r)])[p.j] = _Float16(y - float(hi));
   }
   if constexpr (C::kBits == 4) {  // 16 / G threads hold a block's 32 dims
 #pragma unroll
     for (int o = 1; o < 16 / G; o <<= 1) sum += __shfl_xor(sum, o);
-    if (s % (16u / G) == 0u) q.sum[s / (16u / G)][r] = ldexpf(sum, -24);
+    const uint32_t block = s / (16u / G);
+    if (s % (16u / G) == 0u) q.sum[block % H][r * F + block / H] = ldexpf(sum, -24);
   }
-  if (s == 0u) q.factor[r] = ldexpf(a.scale, (C::kBits == 4 ? 24 : 0) - up);
+  if (s < uint32_t(F)) q.factor[r * F + s] = ldexpf(a.scale, (C::kBits == 4 ? 24 : 0) - up);
 }
 
 // ---- scores ------------------------------------------------------------------------
@@ -499,33 +575,33 @@ __device__ __forceinline__ void tile_scores(const typename C::K& k, const QBlock
   constexpr int G = C::kGroups;
   const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
   if constexpr (C::kBits == 4) {
-    constexpr int PW = C::kPWords;
-    float st[PW], le[PW];
-#pragma unroll
-    for (int i = 0; i < PW; ++i) {
-      st[i] = __uint_as_float(k.p.w[i] & 0xffff0000u);
-      le[i] = __uint_as_float(k.p.w[i] << 16);
-    }
+    constexpr int H = C::kH, F = C::kF;
+    const typename C::Params p = C::template unpack<false>(k.p);
 #pragma unroll
     for (int j = 0; j < 8; ++j) x[j] = 0.f;
-    unrolled<0, G>([&](auto gc) {
-      constexpr int g = gc;
-      const f16x8 ka = C::template k_frag<g>(k.a), kb = C::template k_frag<g>(k.b);
+    unrolled<0, H>([&](auto hc) {
+      constexpr int h = hc;
       f32x4 da = zero, db = zero;
+      unrolled<0, F>([&](auto fc) {
+        constexpr int g = fc * H + h;
+        const f16x8 ka = C::template k_frag<g>(k.a), kb = C::template k_frag<g>(k.b);
 #pragma unroll
-      for (int i = 0; i < QD; ++i) {
-        const f16x8 qd = q.d[g][i][lane];
-        da = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qd, da, 0, 0, 0);
-        db = __builtin_amdgcn_mfma_f32_16x16x32_f16(kb, qd, db, 0, 0, 0);
-      }
-      const float sum = q.sum[g][lane % 16u];
+        for (int i = 0; i < QD; ++i) {
+          const f16x8 qd = q.d[g][i][lane];
+          da = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qd, da, 0, 0, 0);
+          db = __builtin_amdgcn_mfma_f32_16x16x32_f16(kb, qd, db, 0, 0, 0);
+        }
+      });
+      const float sum = q.sum[h][lane % 16u];
       unrolled<0, 8>([&](auto jc) {
-        constexpr int j = jc, from = 2 * j + g / PW, i = g % PW;
+        constexpr int j = jc;
         const float d = j < 4 ? da[j % 4] : db[j % 4];
-        x[j] = fmaf(bc<from>(st[i]), d, x[j]);
-        x[j] = fmaf(bc<from>(le[i]), sum, x[j]);
+        x[j] = fmaf(p.template step_of<j, h>(), d, x[j]);
+        x[j] = fmaf(p.template other_of<j, h>(), sum, x[j]);
       });
     });
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = lanes_sum<F>(x[j]);
   } else {
     f32x4 da = zero, db = zero;
     unrolled<0, G>([&](auto gc) {

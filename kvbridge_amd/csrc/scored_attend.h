@@ -48,34 +48,44 @@ __device__ __forceinline__ void store_out4(const ScoredArgs& a, uint64_t at, f32
   }
 }
 
-// Running state of a wave: acc[f] columns are head-rows, rows dims.
+// Running state of a wave: acc[f] columns are head-rows (times F), rows dims.
+// The reference is kept in units of log 2, where it is exact by definition: p =
+// exp2(fma(score, log2 e, -mref2)) rounds once.
 template <class C>
 struct AttendState {
   f32x4 acc[2 * C::kGroups];
-  float mid[C::kBits == 4 ? C::kGroups : 1];
-  float mref, mtop, l, vf;  // reference, maximum of the lane's scores, sum, 2^ve
+  float mid[C::kBits == 4 ? C::kH : 1];
+  float mref2, mtop, l, vf;  // reference, maximum of the lane's scores, sum, 2^ve
   int ve;
 };
+__device__ __forceinline__ float weight(float score, float mref2) {
+  return __builtin_amdgcn_exp2f(fmaf(score, kLog2e, -mref2));
+}
+// exp(top) / 2^mref2 inverted: the factor from the reference to `top`, with the
+// rounding of top * log2 e taken back.
+__device__ __forceinline__ float to_top(float mref2, float top) {
+  const float t2 = top * kLog2e;
+  return __builtin_amdgcn_exp2f((mref2 - t2) - fmaf(top, kLog2e, -t2));
+}
 
 // Moves the reference to the head-row's maximum and sets ve by the tile's
-// largest weight.  mult(j): the largest step of the lane's token j.
+// largest weight of the column.  mult(j): the largest step of the lane's token j.
 template <class C, typename F>
 __device__ __forceinline__ void rescale(AttendState<C>& s, const float (&x)[8], F mult) {
-  const float top = rows_max(s.mtop);
-  const float mref = fmaxf(s.mref, top);
-  const float jump = mref - s.mref;
-  const float alpha = exp_e(-jump);
+  const float mref2 = fmaxf(s.mref2, rows_max(s.mtop) * kLog2e);
+  const float jump = mref2 - s.mref2;
+  const float alpha = __builtin_amdgcn_exp2f(-jump);
   float w = 0.f;
   unrolled<0, 8>([&](auto jc) {
     constexpr int j = jc;
-    const float p = exp_e(x[j] - mref), big = mult(jc);
+    const float p = weight(x[j], mref2), big = mult(jc);
     w = fmaxf(w, p > 0.f ? p * big : 0.f);
   });
   w = rows_max(w);
   int ve = s.ve;
   if (w > 0.f && w <= FLT_MAX) {
     // Upwards only as far as the reference moved: the numerators must not grow.
-    const int room = s.ve + int(fminf(jump * 1.4375f, 200.f));
+    const int room = s.ve + int(fminf(jump, 200.f));
     ve = -__builtin_amdgcn_frexp_expf(w);
     ve = ve < room ? ve : room;
     ve = ve < -120 ? -120 : (ve > 120 ? 120 : ve);
@@ -88,9 +98,9 @@ __device__ __forceinline__ void rescale(AttendState<C>& s, const float (&x)[8], 
   s.l *= alpha;
   if constexpr (C::kBits == 4) {
 #pragma unroll
-    for (int g = 0; g < C::kGroups; ++g) s.mid[g] *= alpha;
+    for (int h = 0; h < C::kH; ++h) s.mid[h] *= alpha;
   }
-  s.mref = mref;
+  s.mref2 = mref2;
   s.ve = ve;
   s.vf = ldexpf(1.f, ve);
 }
@@ -113,29 +123,30 @@ __device__ __forceinline__ PDigits<PD> p_digits(const float (&w)[8]) {
 
 // Whether a tile asks for another reference or scale: p < 2^8 and step * 2^ve
 // <= 2^7 keep every weight below 2^16.  And the rescale itself.
-template <int G>
-__device__ __forceinline__ void keep_range(const typename Cache4<G>::V& v, const float (&x)[8], AttendState<Cache4<G>>& s) {
-  constexpr int PW = Cache4<G>::kPWords;
-  float st[PW], top = 0.f;
+template <int G, int F>
+__device__ __forceinline__ void keep_range(const typename Cache4<G, F>::V& v, const float (&x)[8], AttendState<Cache4<G, F>>& s) {
+  using C = Cache4<G, F>;
+  typename C::Params p;
+  float top = 0.f;
 #pragma unroll
-  for (int i = 0; i < PW; ++i) {
-    st[i] = __uint_as_float(v.p.w[i] & 0xffff0000u);
-    top = fmaxf(top, st[i]);
+  for (int i = 0; i < C::kPWords; ++i) {
+    p.step[i] = __uint_as_float(v.p.w[i] & 0xffff0000u);
+    top = fmaxf(top, p.step[i]);
   }
-  if (!__any(s.mtop > s.mref + 5.5f || top * s.vf > 128.f)) return;
+  if (!__any(fmaf(s.mtop, kLog2e, -s.mref2) > 8.f || top * s.vf > 128.f)) return;
   rescale(s, x, [&](auto jc) {
     constexpr int j = jc;
     float t = 0.f;
-    unrolled<0, G>([&](auto gc) {
-      constexpr int g = gc, lane = 2 * j + g / PW, i = g % PW;
-      t = fmaxf(t, bc<lane>(st[i]));
+    unrolled<0, C::kH>([&](auto hc) {
+      constexpr int h = hc;
+      t = fmaxf(t, p.template step_of<j, h>());
     });
     return t;
   });
 }
 template <int G>
 __device__ __forceinline__ void keep_range(const typename Cache8<G>::V& v, const float (&x)[8], AttendState<Cache8<G>>& s) {
-  if (!__any(s.mtop > s.mref + 5.5f || v.p * s.vf > 128.f)) return;
+  if (!__any(fmaf(s.mtop, kLog2e, -s.mref2) > 8.f || v.p * s.vf > 128.f)) return;
   rescale(s, x, [&](auto jc) {
     constexpr int j = jc;
     return bc<j>(v.p);
@@ -145,10 +156,11 @@ __device__ __forceinline__ void keep_range(const typename Cache8<G>::V& v, const
 // A tile in which some head-row does not see every token: an infinite or NaN
 // parameter times the weight 0 would reach that head-row.  Such parameters
 // become 0, and the head-rows that do see the token get a NaN in its block.
-template <int G>
-__device__ __forceinline__ void hide_odd_params(typename Cache4<G>::V& v, const float (&x)[8], AttendState<Cache4<G>>& s,
-                                                uint32_t kg) {
-  constexpr int PW = Cache4<G>::kPWords;
+template <int G, int F>
+__device__ __forceinline__ void hide_odd_params(typename Cache4<G, F>::V& v, const float (&x)[8],
+                                                AttendState<Cache4<G, F>>& s, uint32_t kg) {
+  using C = Cache4<G, F>;
+  constexpr int PW = C::kPWords;
   bool odd[PW], any = false;
 #pragma unroll
   for (int i = 0; i < PW; ++i) {
@@ -156,74 +168,82 @@ __device__ __forceinline__ void hide_odd_params(typename Cache4<G>::V& v, const 
     any = any || odd[i];
   }
   if (!__any(any)) return;
-  uint32_t seen = 0u;  // bit 2 j: the lane's token j has a weight
+  const float nan = __builtin_nanf("");
+  if constexpr (F == 1) {
+    uint32_t seen = 0u;  // bit 2 j: the lane's token j has a weight
 #pragma unroll
-  for (int j = 0; j < 8; ++j) seen |= exp_e(x[j] - s.mref) != 0.f ? 1u << (2 * j) : 0u;
+    for (int j = 0; j < 8; ++j) seen |= weight(x[j], s.mref2) != 0.f ? 1u << (2 * j) : 0u;
 #pragma unroll
-  for (int i = 0; i < PW; ++i) {
-    const uint32_t lanes = uint32_t(__ballot(odd[i]) >> (16u * kg));  // bit 2 j + h: token j, block h * PW + i
-    s.mid[i] = (lanes & seen) != 0u ? __builtin_nanf("") : s.mid[i];
-    s.mid[PW + i] = ((lanes >> 1) & seen) != 0u ? __builtin_nanf("") : s.mid[PW + i];
-    v.p.w[i] = odd[i] ? 0u : v.p.w[i];
+    for (int i = 0; i < PW; ++i) {
+      const uint32_t lanes = uint32_t(__ballot(odd[i]) >> (16u * kg));  // bit 2 j + h: token j, block h * PW + i
+      s.mid[i] = (lanes & seen) != 0u ? nan : s.mid[i];
+      s.mid[PW + i] = ((lanes >> 1) & seen) != 0u ? nan : s.mid[PW + i];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < PW; ++i)
+      s.mid[i % C::kH] = odd[i] && weight(x[i / C::kH], s.mref2) != 0.f ? nan : s.mid[i % C::kH];
   }
+#pragma unroll
+  for (int i = 0; i < PW; ++i) v.p.w[i] = odd[i] ? 0u : v.p.w[i];
 }
 template <int G>
 __device__ __forceinline__ void hide_odd_params(typename Cache8<G>::V&, const float (&)[8], AttendState<Cache8<G>>&, uint32_t) {}
 
-// One tile's weights and their products with V.
-template <int G, int PD>
-__device__ __forceinline__ void tile_values(const typename Cache4<G>::V& v, const float (&x)[8], AttendState<Cache4<G>>& s) {
-  constexpr int PW = Cache4<G>::kPWords;
-  float st[PW], mid[PW];
-#pragma unroll
-  for (int i = 0; i < PW; ++i) {
-    st[i] = __uint_as_float(v.p.w[i] & 0xffff0000u);
-    mid[i] = fmaf(st[i], 8.f, __uint_as_float(v.p.w[i] << 16));
-  }
+// One tile's weights and their products with V.  code_bits: 1024 as two fp16,
+// held in a register (an instruction takes one constant, the mask).
+template <int PD, int G, int F>
+__device__ __forceinline__ void tile_values(const typename Cache4<G, F>::V& v, const float (&x)[8],
+                                            AttendState<Cache4<G, F>>& s, uint32_t code_bits) {
+  using C = Cache4<G, F>;
+  const typename C::Params par = C::template unpack<true>(v.p);
   float p[8], pv[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    p[j] = exp_e(x[j] - s.mref);
+    p[j] = weight(x[j], s.mref2);
     pv[j] = p[j] * s.vf;
   }
   s.l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-  unrolled<0, G>([&](auto gc) {
-    constexpr int g = gc;
+  unrolled<0, C::kH>([&](auto hc) {
+    constexpr int h = hc;
     float w[8];
     unrolled<0, 8>([&](auto jc) {
-      constexpr int j = jc, lane = 2 * j + g / PW, i = g % PW;
-      const float step = bc<lane>(st[i]), at8 = bc<lane>(mid[i]);
+      constexpr int j = jc;
+      const float step = par.template step_of<j, h>(), at8 = par.template other_of<j, h>();
       w[j] = step * pv[j];
-      s.mid[g] = fmaf(at8, p[j], s.mid[g]);
+      s.mid[h] = fmaf(at8, p[j], s.mid[h]);
     });
     const PDigits<PD> d = p_digits<PD>(w);
-    uint32_t u[4];
+    unrolled<0, F>([&](auto fc) {
+      constexpr int g = fc * C::kH + h;
+      uint32_t u[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      constexpr uint32_t sel = 0x0c000c00u | uint32_t(g % 4) | uint32_t(4 + g % 4) << 16;
-      u[i] = __builtin_amdgcn_perm(v.v[2 * i + 1].w[g / 4], v.v[2 * i].w[g / 4], sel);
-    }
-    // 1024 + c and 1024 + 16 c as fp16 bits, less 1032 and 1152
-    f16x8 even = as_f16x8((u[0] & 0x000f000fu) | 0x64006400u, (u[1] & 0x000f000fu) | 0x64006400u,
-                          (u[2] & 0x000f000fu) | 0x64006400u, (u[3] & 0x000f000fu) | 0x64006400u);
-    f16x8 odd = as_f16x8((u[0] & 0x00f000f0u) | 0x64006400u, (u[1] & 0x00f000f0u) | 0x64006400u,
-                         (u[2] & 0x00f000f0u) | 0x64006400u, (u[3] & 0x00f000f0u) | 0x64006400u);
-    even -= (_Float16)1032.f;
-    odd -= (_Float16)1152.f;
+      for (int i = 0; i < 4; ++i) {
+        constexpr uint32_t sel = 0x0c000c00u | uint32_t(g % 4) | uint32_t(4 + g % 4) << 16;
+        u[i] = __builtin_amdgcn_perm(v.v[2 * i + 1].w[g / 4], v.v[2 * i].w[g / 4], sel);
+      }
+      // 1024 + c and 1024 + 16 c as fp16 bits, less 1032 and 1152
+      const uint32_t m = code_bits;
+      f16x8 even = as_f16x8((u[0] & 0x000f000fu) | m, (u[1] & 0x000f000fu) | m, (u[2] & 0x000f000fu) | m, (u[3] & 0x000f000fu) | m);
+      f16x8 odd = as_f16x8((u[0] & 0x00f000f0u) | m, (u[1] & 0x00f000f0u) | m, (u[2] & 0x00f000f0u) | m, (u[3] & 0x00f000f0u) | m);
+      even -= (_Float16)1032.f;
+      odd -= (_Float16)1152.f;
 #pragma unroll
-    for (int i = 0; i < PD; ++i) {
-      s.acc[2 * g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, d.d[i], s.acc[2 * g], 0, 0, 0);
-      s.acc[2 * g + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, d.d[i], s.acc[2 * g + 1], 0, 0, 0);
-    }
-    __builtin_amdgcn_sched_barrier(0);  // one block's operands at a time in registers
+      for (int i = 0; i < PD; ++i) {
+        s.acc[2 * g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, d.d[i], s.acc[2 * g], 0, 0, 0);
+        s.acc[2 * g + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, d.d[i], s.acc[2 * g + 1], 0, 0, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);  // one block's operands at a time in registers
+    });
   });
 }
-template <int G, int PD>
-__device__ __forceinline__ void tile_values(const typename Cache8<G>::V& v, const float (&x)[8], AttendState<Cache8<G>>& s) {
+template <int PD, int G>
+__device__ __forceinline__ void tile_values(const typename Cache8<G>::V& v, const float (&x)[8], AttendState<Cache8<G>>& s,
+                                            uint32_t) {
   float p[8], w[8];
   unrolled<0, 8>([&](auto jc) {
     constexpr int j = jc;
-    p[j] = exp_e(x[j] - s.mref);
+    p[j] = weight(x[j], s.mref2);
     w[j] = bc<j>(v.p) * (p[j] * s.vf);
     w[j] = p[j] == 0.f ? 0.f : w[j];
   });
@@ -237,23 +257,32 @@ __device__ __forceinline__ void tile_values(const typename Cache8<G>::V& v, cons
   }
 }
 
-// Four consecutive dims of a head-row in units of exp(mref): chunk c of
-// 2 G, and the first of its dims.
-template <int G>
-__device__ __forceinline__ f32x4 chunk_value(const AttendState<Cache4<G>>& s, int c, const float (&mid)[G]) {
-  const int g = c / 2, h = c % 2;
+// Four consecutive dims of a lane's head-row in units of 2^mref2: chunk c of its
+// 2 H, and the first of its dims.
+template <int G, int F>
+__device__ __forceinline__ f32x4 chunk_value(const AttendState<Cache4<G, F>>& s, int c, const float (&mid)[G / F], uint32_t r) {
+  constexpr int H = G / F;
+  const int h = c / 2, half = c % 2;
+  f32x4 a = s.acc[2 * h], o = s.acc[2 * h + 1];  // even and odd dims of the lane's block f * H + h
+#pragma unroll
+  for (int f = 1; f < F; ++f)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      a[i] = r % F == uint32_t(f) ? s.acc[2 * (f * H + h)][i] : a[i];
+      o[i] = r % F == uint32_t(f) ? s.acc[2 * (f * H + h) + 1][i] : o[i];
+    }
   const float even = ldexpf(1.f, -s.ve), odd = ldexpf(1.f, -4 - s.ve);
-  return f32x4{fmaf(s.acc[2 * g][2 * h], even, mid[g]), fmaf(s.acc[2 * g + 1][2 * h], odd, mid[g]),
-               fmaf(s.acc[2 * g][2 * h + 1], even, mid[g]), fmaf(s.acc[2 * g + 1][2 * h + 1], odd, mid[g])};
+  return f32x4{fmaf(a[2 * half], even, mid[h]), fmaf(o[2 * half], odd, mid[h]), fmaf(a[2 * half + 1], even, mid[h]),
+               fmaf(o[2 * half + 1], odd, mid[h])};
 }
 template <int G>
-__device__ __forceinline__ f32x4 chunk_value(const AttendState<Cache8<G>>& s, int c, const float (&)[1]) {
+__device__ __forceinline__ f32x4 chunk_value(const AttendState<Cache8<G>>& s, int c, const float (&)[1], uint32_t) {
   const float f = ldexpf(1.f, -s.ve);
   return f32x4{s.acc[c][0] * f, s.acc[c][1] * f, s.acc[c][2] * f, s.acc[c][3] * f};
 }
 template <class C>
-__device__ __forceinline__ uint32_t chunk_dim(uint32_t c, uint32_t kg) {
-  return C::kBits == 4 ? 32u * (c / 2u) + 8u * kg + 4u * (c % 2u) : 16u * c + 4u * kg;
+__device__ __forceinline__ uint32_t chunk_dim(uint32_t c, uint32_t r, uint32_t kg) {
+  return C::kBits == 4 ? 32u * (r % C::kF * C::kH + c / 2u) + 8u * kg + 4u * (c % 2u) : 16u * c + 4u * kg;
 }
 
 // LDS: Q's operands while the tiles run, then the waves' numerators, eight
@@ -261,12 +290,16 @@ __device__ __forceinline__ uint32_t chunk_dim(uint32_t c, uint32_t kg) {
 template <class C, int QD>
 union AttendLds {
   QBlock<C, QD> q;
-  f32x4 o[kAttendWaves][2 * C::kGroups < 8 ? 2 * C::kGroups : 8][64];
+  f32x4 o[kAttendWaves][2 * C::kH < 8 ? 2 * C::kH : 8][64];
 };
 
+// Waves per SIMD that the registers allow without spills.
+template <class C, bool ONE>
+constexpr int kAttendOccupancy = C::kGroups == 8 || (C::kF > 1 && C::kH > 1) || (C::kBits == 8 && !ONE) ? 2 : 3;
+
 template <class C, int QD, int PD, bool ONE>
-__global__ __launch_bounds__(64 * kAttendWaves, C::kGroups == 8 ? 2 : 3) void scored_attend_kernel(const ScoredArgs a) {
-  constexpr int G = C::kGroups, NC = 2 * G, NW = kAttendWaves, NR = NC < 8 ? NC : 8;
+__global__ __launch_bounds__(64 * kAttendWaves, (kAttendOccupancy<C, ONE>)) void scored_attend_kernel(const ScoredArgs a) {
+  constexpr int F = C::kF, NC = 2 * C::kH, NW = kAttendWaves, NR = NC < 8 ? NC : 8;
   __shared__ AttendLds<C, QD> lds;
   __shared__ float lds_m[NW][16], lds_l[NW][16];
   const uint32_t lane = threadIdx.x & 63u, r = lane & 15u, kg = lane >> 4;
@@ -278,7 +311,7 @@ __global__ __launch_bounds__(64 * kAttendWaves, C::kGroups == 8 ? 2 : 3) void sc
   at /= a.blocks;
   const uint32_t split = at % a.splits, b = at / a.splits;
 
-  const uint32_t hr = block * 16u + r;
+  const uint32_t hr = block * 16u + r / F;  // F > 1: one block
   const bool valid = hr < a.head_rows;
   const uint32_t hrc = valid ? hr : a.head_rows - 1u;
   const uint32_t row = hrc / a.group, head = kv * a.group + hrc % a.group;
@@ -292,7 +325,7 @@ __global__ __launch_bounds__(64 * kAttendWaves, C::kGroups == 8 ? 2 : 3) void sc
   per = per > a.split_tiles ? per : a.split_tiles;
   const uint32_t own = live.n > 0u ? (live.n - 1u) / per + 1u : 1u;
   if (split >= own) {
-    if (a.splits > 1u && wave == 0u && valid && kg == 0u) {
+    if (a.splits > 1u && wave == 0u && valid && kg == 0u && r % F == 0u) {
       float* ml = partial_place(a, rh, split).ml;
       ml[0] = neg_inf();
       ml[1] = 0.f;
@@ -310,10 +343,10 @@ __global__ __launch_bounds__(64 * kAttendWaves, C::kGroups == 8 ? 2 : 3) void sc
 
   AttendState<C> s;
 #pragma unroll
-  for (int f = 0; f < NC; ++f) s.acc[f] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int f = 0; f < 2 * C::kGroups; ++f) s.acc[f] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int g = 0; g < (C::kBits == 4 ? G : 1); ++g) s.mid[g] = 0.f;
-  s.mref = -FLT_MAX;
+  for (int h = 0; h < (C::kBits == 4 ? C::kH : 1); ++h) s.mid[h] = 0.f;
+  s.mref2 = -FLT_MAX;
   s.mtop = neg_inf();
   s.l = 0.f;
   s.vf = 1.f;
@@ -326,6 +359,8 @@ __global__ __launch_bounds__(64 * kAttendWaves, C::kGroups == 8 ? 2 : 3) void sc
     const uint64_t t = uint64_t(first) + uint64_t(i) * NW;
     return live.tile(t < live.n ? uint32_t(t) : live.n - 1u);
   };
+  uint32_t code_bits = 0x64006400u;
+  asm("" : "+v"(code_bits));
   if (n > 0u) {
     TilePages pages = tile_pages(a, e, tile_of, 0u, lane), ahead_pages = pages;
     TileRows<ONE> rows = tile_rows<ONE>(a, pages, 0u, kv);
@@ -346,9 +381,9 @@ __global__ __launch_bounds__(64 * kAttendWaves, C::kGroups == 8 ? 2 : 3) void sc
       const bool whole = t0 + kTileTokens <= vis.pre || (t0 >= vis.all_lo && t0 + kTileTokens <= vis.all_hi);
       apply_form<C>(a, form, ahead, t0, kg, !whole, vis.lo, vis.hi, vis.pre, x);
       s.mtop = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])), s.mtop));
-      keep_range<G>(v, x, s);
-      if (!whole) hide_odd_params<G>(v, x, s, kg);
-      tile_values<G, PD>(v, x, s);
+      keep_range(v, x, s);
+      if (!whole) hide_odd_params(v, x, s, kg);
+      tile_values<PD>(v, x, s, code_bits);
       k = k_next;
       rows = rows_next;
       t0 = t_next;
@@ -359,41 +394,39 @@ __global__ __launch_bounds__(64 * kAttendWaves, C::kGroups == 8 ? 2 : 3) void sc
   // The waves' parts: a common maximum, then each wave adds a quarter of the dims.
   const float l = rows_sum(s.l), mtop = rows_max(s.mtop);
   if (kg == 0u) lds_m[wave][r] = mtop;
-  float mid[C::kBits == 4 ? G : 1];
+  float mid[C::kBits == 4 ? C::kH : 1];
 #pragma unroll
-  for (int g = 0; g < (C::kBits == 4 ? G : 1); ++g) mid[g] = rows_sum(s.mid[g]);
+  for (int h = 0; h < (C::kBits == 4 ? C::kH : 1); ++h) mid[h] = rows_sum(s.mid[h]);
   __syncthreads();  // also: every wave is done with Q
   float top = lds_m[0][r];
 #pragma unroll
   for (int w = 1; w < NW; ++w) top = fmaxf(top, lds_m[w][r]);
-  // A wave without visible tokens has mref = -FLT_MAX: a factor of 0.
-  const float f = l == 0.f ? 0.f : exp_e(s.mref - top);
+  const float f = l == 0.f ? 0.f : to_top(s.mref2, top);  // a wave without visible tokens: 0
   if (kg == 0u) lds_l[wave][r] = l * f;
   const bool done = own == 1u;
   const PartialPlace part = done ? PartialPlace{nullptr, nullptr} : partial_place(a, rh, split);
-  float sum = 0.f;
 #pragma unroll
   for (int round = 0; round < NC / NR; ++round) {
 #pragma unroll
     for (int c = 0; c < NR; ++c) {
-      f32x4 o = chunk_value(s, round * NR + c, mid);
+      f32x4 o = chunk_value(s, round * NR + c, mid, r);
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[i] = l == 0.f ? 0.f : o[i] * f;
       lds.o[wave][c][lane] = o;
     }
     __syncthreads();
-    if (round == 0) {
+    // Wave w: chunks w, w + 4 (a wave's lanes are the tiles' lanes again).
 #pragma unroll
-      for (int w = 0; w < NW; ++w) sum += lds_l[w][r];
-    }
-#pragma unroll
-    for (int i = 0; i < NR / NW; ++i) {
-      const uint32_t c = wave * (NR / NW) + i;
+    for (uint32_t c = wave; c < uint32_t(NR); c += NW) {
       f32x4 o = lds.o[0][c][lane];
+      float sum = lds_l[0][r];
 #pragma unroll
-      for (int w = 1; w < NW; ++w) o += lds.o[w][c][lane];
+      for (int w = 1; w < NW; ++w) {
+        o += lds.o[w][c][lane];
+        sum += lds_l[w][r];
+      }
       if (!valid) continue;
-      const uint32_t d = chunk_dim<C>(round * NR + c, kg);
+      const uint32_t d = chunk_dim<C>(round * NR + c, r, kg);
       if (done) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) o[k] = sum == 0.f ? 0.f : o[k] / sum;
@@ -404,7 +437,10 @@ __global__ __launch_bounds__(64 * kAttendWaves, C::kGroups == 8 ? 2 : 3) void sc
     }
     if (round + 1 < NC / NR) __syncthreads();
   }
-  if (wave == 0u && valid && kg == 0u) {
+  float sum = lds_l[0][r];
+#pragma unroll
+  for (int w = 1; w < NW; ++w) sum += lds_l[w][r];
+  if (wave == 0u && valid && kg == 0u && r % F == 0u) {
     if (done) {
       a.m[rh] = sum == 0.f ? neg_inf() : top;
       a.l[rh] = sum;
@@ -467,10 +503,21 @@ inline hipError_t launch_attend_kernel(const ScoredArgs& a, hipStream_t stream) 
 // Weights of one digit only where the output is bf16 and q has 16 bits.
 template <class C>
 inline hipError_t launch_attend_cache(const ScoredArgs& a, hipStream_t stream) {
-  if (a.q_type == 1u) return launch_attend_kernel<C, 2, 2>(a, stream);
   constexpr int QD = kQDigits<C, false>;
+  if (a.q_type == 1u) return launch_attend_kernel<C, 2, 2>(a, stream);
   if (a.out_type == 3u) return launch_attend_kernel<C, QD, 1>(a, stream);
   return launch_attend_kernel<C, QD, 2>(a, stream);
+}
+// As many columns per head-row as there is room for, up to one per block (two
+// blocks per column at the least F > 1: with more the parameters take too many
+// registers).
+template <int G>
+inline hipError_t launch_attend_cache4(const ScoredArgs& a, hipStream_t stream) {
+  if (a.head_rows <= 16u / G) return launch_attend_cache<Cache4<G, G>>(a, stream);
+  if constexpr (G > 2) {
+    if (a.head_rows <= 32u / G) return launch_attend_cache<Cache4<G, G / 2>>(a, stream);
+  }
+  return launch_attend_cache<Cache4<G, 1>>(a, stream);
 }
 
 hipError_t launch_attend4_d64(const ScoredArgs& a, hipStream_t stream);

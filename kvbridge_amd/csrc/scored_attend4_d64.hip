@@ -2,7 +2,5 @@
 #include "scored_attend.h"
 
 namespace kvb {
-hipError_t launch_attend4_d64(const ScoredArgs& a, hipStream_t stream) {
-  return launch_attend_cache<Cache4<2>>(a, stream);
-}
+hipError_t launch_attend4_d64(const ScoredArgs& a, hipStream_t stream) { return launch_attend_cache4<2>(a, stream); }
 }  // namespace kvb

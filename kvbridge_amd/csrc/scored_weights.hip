@@ -68,7 +68,7 @@ __global__ __launch_bounds__(64 * kWeightWaves) void scored_weights_kernel(const
     }
     uint32_t pre = 0;
     for (uint32_t i = wave; i < count; i += kWeightWaves) {
-      const uint32_t hr = (first + i) * 16u + r;
+      const uint32_t hr = (first + i) * 16u + r / C::kF;
       const bool valid = hr < a.head_rows;
       const uint32_t hrc = valid ? hr : a.head_rows - 1u;
       const uint32_t row = hrc / a.group, head = kv * a.group + hrc % a.group;
@@ -82,7 +82,7 @@ __global__ __launch_bounds__(64 * kWeightWaves) void scored_weights_kernel(const
         w.lo[r] = vis.lo;
         w.hi[r] = vis.hi;
         w.m[r] = counts ? a.m[rh] : FLT_MAX;
-        w.per_l[r] = counts ? 1.f / l : 0.f;
+        w.per_l[r] = counts && r % C::kF == 0u ? 1.f / l : 0.f;  // a head-row's F columns hold the same score
         w.slope[r] = a.slopes ? a.slopes[head] : 0.f;
         w.back[r] = near(int64_t(uint64_t(qpos) - uint64_t(qref)));
       }
@@ -191,13 +191,22 @@ hipError_t launch_cache(const ScoredArgs& a, hipStream_t stream) {
   return launch_digits<C, kQDigits<C, false>>(a, stream);
 }
 
+template <int G>
+hipError_t launch_cache4(const ScoredArgs& a, hipStream_t stream) {  // as launch_attend_cache4
+  if (a.head_rows <= 16u / G) return launch_cache<Cache4<G, G>>(a, stream);
+  if constexpr (G > 2) {
+    if (a.head_rows <= 32u / G) return launch_cache<Cache4<G, G / 2>>(a, stream);
+  }
+  return launch_cache<Cache4<G, 1>>(a, stream);
+}
+
 }  // namespace
 
 hipError_t launch_scored_weights(const ScoredArgs& a, hipStream_t stream) {
   if (a.kv_bits == 4u) {
-    if (a.dim == 64u) return launch_cache<Cache4<2>>(a, stream);
-    if (a.dim == 128u) return launch_cache<Cache4<4>>(a, stream);
-    return launch_cache<Cache4<8>>(a, stream);
+    if (a.dim == 64u) return launch_cache4<2>(a, stream);
+    if (a.dim == 128u) return launch_cache4<4>(a, stream);
+    return launch_cache4<8>(a, stream);
   }
   if (a.dim == 64u) return launch_cache<Cache8<2>>(a, stream);
   if (a.dim == 128u) return launch_cache<Cache8<4>>(a, stream);
