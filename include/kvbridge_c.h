@@ -306,8 +306,9 @@ typedef struct kvb_scored_input {
   const int64_t* prefix; /* [batch] or NULL */
 } kvb_scored_input;
 const char* kvb_scored_shape_error(const kvb_scored_shape* s);
-/* Splits of one sequence (partials in scratch). */
-int kvb_scored_split_count(const kvb_scored_shape* s, uint32_t* splits);
+/* Work items of a kv head, each a part of one sequence with its partials in
+ * scratch. */
+int kvb_scored_item_count(const kvb_scored_shape* s, uint32_t* items);
 int kvb_scored_scratch_elements(const kvb_scored_shape* s, size_t* elements);
 int kvb_scored_counter_elements(const kvb_scored_shape* s, size_t* elements);
 int kvb_decode_attention_scored(const kvb_scored_shape* s, const kvb_scored_input* in, float* scratch,

@@ -348,9 +348,9 @@ def scored_shape_error(s: ScoredShape):
     return None if r is None else r.decode()
 
 
-def scored_split_count(s: ScoredShape) -> int:
+def scored_item_count(s: ScoredShape) -> int:
     out = ctypes.c_uint32()
-    check(load().kvb_scored_split_count(ctypes.byref(s), ctypes.byref(out)))
+    check(load().kvb_scored_item_count(ctypes.byref(s), ctypes.byref(out)))
     return out.value
 
 

@@ -223,7 +223,7 @@ SIGNATURES = [
     ("kvb_read_shape_error", ctypes.c_char_p, [ctypes.POINTER(ReadShape)]),
     ("kvb_read_kv", _INT, [ctypes.POINTER(ReadShape), ctypes.POINTER(ReadIO), _VP]),
     ("kvb_scored_shape_error", ctypes.c_char_p, [_SSP]),
-    ("kvb_scored_split_count", _INT, [_SSP, ctypes.POINTER(_U32)]),
+    ("kvb_scored_item_count", _INT, [_SSP, ctypes.POINTER(_U32)]),
     ("kvb_scored_scratch_elements", _INT, [_SSP, ctypes.POINTER(ctypes.c_size_t)]),
     ("kvb_scored_counter_elements", _INT, [_SSP, ctypes.POINTER(ctypes.c_size_t)]),
     ("kvb_decode_attention_scored", _INT, [_SSP, _SIP, _VP, _VP, _VP, _VP, _VP, _INT, _VP]),

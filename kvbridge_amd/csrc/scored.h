@@ -46,6 +46,7 @@
 #include <cfloat>
 #include <cstdint>
 
+#include "batch.h"
 #include "device_common.h"
 #include "scored_args.h"
 
@@ -90,14 +91,137 @@ __device__ __forceinline__ ScoredSeq clamp_seq(uint32_t s0, uint32_t s1, uint32_
   return ScoredSeq{s0, t, off};
 }
 
+// A work-group's part of the batch: split `split` of the `count` that sequence
+// `seq` has, whose items begin at `first`.
+struct WorkItem {
+  uint32_t seq, split, count, first;
+  ScoredSeq e;
+};
+__device__ __forceinline__ ScoredSeq load_seq(const ScoredArgs& a, uint32_t b) {
+  return clamp_seq(a.seq_starts[b], a.seq_starts[b + 1u], a.page_offsets[b], a.total_tokens, a.table_entries, a.page_tokens,
+                   a.max_tokens);
+}
+
+// How many items each sequence gets where the host leaves that open (at most
+// 256 sequences, four per lane): one, and of its tiles a share that is the same
+// for all and as large as the number of items allows.  Every wave of the call,
+// and of the merge, derives the same numbers from the same metadata.
+struct ItemShares {
+  uint32_t count[4];
+};
+__device__ __forceinline__ ItemShares item_shares(const ScoredArgs& a) {
+  const uint32_t lane = threadIdx.x & 63u;
+  ItemShares s;
+  float tiles[4], total = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t b = 64u * i + lane;
+    tiles[i] = 0.f;
+    if (64u * i < a.batch && b < a.batch) {
+      const uint32_t t = load_seq(a, b).tokens;
+      const uint64_t seen = uint64_t(a.window) + a.rows + 31u;
+      uint32_t n = (a.window != 0u && seen < t ? uint32_t(seen) : t) / kTileTokens + 1u;
+      if (a.prefix != nullptr && a.window != 0u) {
+        const int64_t p = a.prefix[b];
+        n += p <= 0 ? 0u : (p < int64_t(t) ? uint32_t(p) : t) / kTileTokens + 1u;
+      }
+      tiles[i] = float(n);
+    }
+    total += tiles[i];
+  }
+  total = wave_sum(total);
+  float per = fminf(1.f / float(a.split_tiles), float(a.items) / total);  // items per tile
+  for (int round = 0; round < 24; ++round) {
+    uint32_t n = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t b = 64u * i + lane;
+      const uint32_t c = uint32_t(tiles[i] * per + 0.9990234375f);
+      s.count[i] = b < a.batch ? (c > 1u ? c : 1u) : 0u;
+      n += s.count[i];
+    }
+    n = uint32_t(__builtin_amdgcn_readlane(int(wave_scan(n)), 63));
+    if (n <= a.items) return s;
+    per = round < 22 ? per * (0.999f * float(a.items) / float(n)) : 0.f;  // at last one item each
+  }
+  return s;
+}
+
+// Item w's sequence and split; false past the last item.
+__device__ __forceinline__ bool item_of(const ScoredArgs& a, uint32_t w, WorkItem& it) {
+  if (a.splits != 0u) {
+    it.seq = w / a.splits;
+    it.split = w - it.seq * a.splits;
+    it.count = a.splits;
+    it.first = w - it.split;
+    it.e = load_seq(a, it.seq);
+    return true;
+  }
+  const ItemShares s = item_shares(a);
+  uint32_t base = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (64u * i >= a.batch) break;
+    const uint32_t upto = base + wave_scan(s.count[i]);
+    const uint64_t hit = __ballot(upto > w);
+    if (hit != 0u) {
+      const int l = __builtin_ctzll(hit);
+      it.seq = 64u * i + uint32_t(l);
+      it.count = uint32_t(__builtin_amdgcn_readlane(int(s.count[i]), l));
+      it.first = uint32_t(__builtin_amdgcn_readlane(int(upto), l)) - it.count;
+      it.split = w - it.first;
+      it.e = load_seq(a, it.seq);
+      return true;
+    }
+    base = uint32_t(__builtin_amdgcn_readlane(int(upto), 63));
+  }
+  return false;
+}
+// The items of sequence b: first and count.
+__device__ __forceinline__ WorkItem items_of(const ScoredArgs& a, uint32_t b) {
+  WorkItem it;
+  it.seq = b;
+  it.split = 0u;
+  it.count = a.splits;
+  it.first = b * a.splits;
+  if (a.splits != 0u) return it;
+  const ItemShares s = item_shares(a);
+  uint32_t base = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t upto = base + wave_scan(s.count[i]);
+    if (b / 64u == uint32_t(i)) {
+      it.count = uint32_t(__builtin_amdgcn_readlane(int(s.count[i]), int(b % 64u)));
+      it.first = uint32_t(__builtin_amdgcn_readlane(int(upto), int(b % 64u))) - it.count;
+    }
+    base = uint32_t(__builtin_amdgcn_readlane(int(upto), 63));
+  }
+  return it;
+}
+
 // First t in [0, n) with kpos[t] > x, else n (kpos nondecreasing), by every
-// lane for its own x.  Positions mostly count up by one, so the place that
-// this implies from the last position is tried first: one round of loads
-// instead of a search's seventeen.
-__device__ __forceinline__ uint32_t first_above(const int64_t* __restrict__ kpos, uint32_t n, int64_t last, int64_t x) {
+// lane for its own x.  The first guess is that positions count up from 0: its
+// two neighbours are requested beside the last position, before any of them is
+// waited for.  Next the place that the last position implies if they count up
+// by one, then a search.
+struct Above {
+  int64_t x, above, below;
+  uint32_t g;
+};
+__device__ __forceinline__ Above ask_above(const int64_t* __restrict__ kpos, uint32_t n, int64_t x) {
+  Above q;
+  q.x = x;
+  q.g = x < 0 ? 0u : (uint64_t(x) + 1u < n ? uint32_t(x) + 1u : (n > 0u ? n - 1u : 0u));
+  q.above = n > 0u ? kpos[q.g] : 0;
+  q.below = n > 0u && q.g > 0u ? kpos[q.g - 1u] : INT64_MIN;
+  return q;
+}
+__device__ __forceinline__ uint32_t find_above(const int64_t* __restrict__ kpos, uint32_t n, int64_t last, const Above& q) {
+  const int64_t x = q.x;
   if (n == 0u || last <= x) return n;
+  if (q.above > x && (q.g == 0u || q.below <= x)) return q.g;
   const uint64_t back = uint64_t(last) - uint64_t(x);  // positive
-  uint32_t g = back < n ? n - uint32_t(back) : 0u;
+  const uint32_t g = back < n ? n - uint32_t(back) : 0u;
   const int64_t above = kpos[g], below = g > 0u ? kpos[g - 1u] : INT64_MIN;
   uint32_t lo = 0, hi = n - 1u;  // kpos[hi] > x
   if (above > x && (g == 0u || below <= x)) return g;
@@ -127,24 +251,32 @@ struct Visible {
   uint32_t lo, hi;
   uint32_t pre, min_lo, max_hi, all_lo, all_hi;
 };
-__device__ __forceinline__ Visible visible_tokens(const ScoredArgs& a, const ScoredSeq& e, uint32_t b, bool valid,
-                                                  int64_t qpos) {
+// What visible_tokens has to look up, requested early.
+struct Sight {
+  int64_t last;
+  Above hi, lo, pre;
+  bool has_lo, has_pre;
+};
+__device__ __forceinline__ Sight ask_visible(const ScoredArgs& a, const ScoredSeq& e, int64_t qpos, int64_t prefix) {
+  const int64_t* kpos = a.k_positions + e.start;
+  Sight s;
+  s.last = e.tokens > 0u ? kpos[e.tokens - 1u] : 0;
+  s.hi = ask_above(kpos, e.tokens, qpos);
+  const int64_t w = int64_t(a.window);
+  s.has_lo = a.window != 0u && qpos >= INT64_MIN + w;  // qpos - kpos < window  <=>  kpos > qpos - window
+  s.has_pre = a.prefix != nullptr && prefix > INT64_MIN;
+  s.lo = s.pre = s.hi;
+  if (a.window != 0u) s.lo = ask_above(kpos, e.tokens, s.has_lo ? qpos - w : INT64_MIN);
+  if (a.prefix != nullptr) s.pre = ask_above(kpos, e.tokens, s.has_pre ? prefix - 1 : INT64_MIN);
+  return s;
+}
+__device__ __forceinline__ Visible visible_tokens(const ScoredArgs& a, const ScoredSeq& e, bool valid, const Sight& s) {
   Visible v;
   const int64_t* kpos = a.k_positions + e.start;
-  const int64_t last = e.tokens > 0u ? kpos[e.tokens - 1u] : 0;
-  v.hi = first_above(kpos, e.tokens, last, qpos);
-  v.lo = 0u;
-  if (a.window != 0u) {
-    const int64_t w = int64_t(a.window);
-    // qpos - kpos < window  <=>  kpos > qpos - window
-    if (qpos >= INT64_MIN + w) v.lo = first_above(kpos, e.tokens, last, qpos - w);
-  }
+  v.hi = find_above(kpos, e.tokens, s.last, s.hi);
+  v.lo = s.has_lo ? find_above(kpos, e.tokens, s.last, s.lo) : 0u;
+  v.pre = s.has_pre ? find_above(kpos, e.tokens, s.last, s.pre) : 0u;
   if (v.lo > v.hi) v.lo = v.hi;
-  v.pre = 0u;
-  if (a.prefix != nullptr) {
-    const int64_t p = a.prefix[b];
-    if (p > INT64_MIN) v.pre = first_above(kpos, e.tokens, last, p - 1);
-  }
   if (!valid) v.lo = v.hi = 0u;
   const bool sees = v.lo < v.hi;
   v.pre = uint32_t(__builtin_amdgcn_readfirstlane(int(v.pre)));
@@ -161,13 +293,16 @@ __device__ __forceinline__ Visible visible_tokens(const ScoredArgs& a, const Sco
 // n - pre_tiles) of the rows' windows, numbered 0 .. n - 1.
 struct LiveTiles {
   uint32_t pre_tiles, first, n;
+  __device__ __forceinline__ bool same(const LiveTiles& o) const {
+    return pre_tiles == o.pre_tiles && first == o.first && n == o.n;
+  }
   __device__ __forceinline__ uint32_t tile(uint32_t i) const { return i < pre_tiles ? i : i - pre_tiles + first; }
 };
-__device__ __forceinline__ LiveTiles live_tiles(const Visible& v) {
+__device__ __forceinline__ LiveTiles live_tiles(uint32_t pre, uint32_t lo, uint32_t hi) {
   LiveTiles t;
-  t.pre_tiles = v.pre / kTileTokens + (v.pre % kTileTokens != 0u ? 1u : 0u);
-  t.first = v.min_lo / kTileTokens;
-  const uint32_t end = v.max_hi / kTileTokens + (v.max_hi % kTileTokens != 0u ? 1u : 0u);
+  t.pre_tiles = pre / kTileTokens + (pre % kTileTokens != 0u ? 1u : 0u);
+  t.first = lo / kTileTokens;
+  const uint32_t end = hi / kTileTokens + (hi % kTileTokens != 0u ? 1u : 0u);
   if (t.first < t.pre_tiles) t.first = t.pre_tiles;
   t.n = t.pre_tiles + (end > t.first ? end - t.first : 0u);
   return t;

@@ -21,17 +21,29 @@ namespace kvb {
 
 constexpr int kAttendWaves = 4;
 
-// Partials: (max score, l) pairs of all splits, then the
-// numerators: scratch[(rh * splits + s) * 2], scratch[2 * rh_total * splits +
-// (rh * splits + s) * dim].  l = -1 in split 0: the result is already written.
+// Partials of item w: (max score, l) pairs of its head-rows, then the
+// numerators: scratch[(w * row_heads + rh) * 2], scratch[2 * items * row_heads +
+// (w * row_heads + rh) * dim], rh = row * q_heads + head.  They are stored and
+// read by agent-scope atomics of 8 bytes, which every XCD sees without a
+// write-back of its L2.
 struct PartialPlace {
   float* ml;
   float* o;
 };
-__device__ __forceinline__ PartialPlace partial_place(const ScoredArgs& a, uint64_t rh, uint32_t split) {
-  const uint64_t all = uint64_t(a.batch) * a.rows * a.q_heads * a.splits;
-  const uint64_t at = rh * a.splits + split;
-  return PartialPlace{a.scratch + at * 2u, a.scratch + all * 2u + at * a.dim};
+__device__ __forceinline__ PartialPlace partial_place(const ScoredArgs& a, uint32_t item, uint32_t rh) {
+  const uint64_t row_heads = uint64_t(a.rows) * a.q_heads, at = item * row_heads + rh;
+  return PartialPlace{a.scratch + at * 2u, a.scratch + a.items * row_heads * 2u + at * a.dim};
+}
+struct Pair {
+  float x, y;
+};
+__device__ __forceinline__ void store_pair(float* p, float x, float y) {
+  const uint64_t v = uint64_t(__float_as_uint(x)) | uint64_t(__float_as_uint(y)) << 32;
+  __hip_atomic_store(reinterpret_cast<uint64_t*>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ Pair load_pair(const float* p) {
+  const uint64_t v = __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return Pair{__uint_as_float(uint32_t(v)), __uint_as_float(uint32_t(v >> 32))};
 }
 
 __device__ __forceinline__ void store_out4(const ScoredArgs& a, uint64_t at, f32x4 o) {
@@ -285,12 +297,117 @@ __device__ __forceinline__ uint32_t chunk_dim(uint32_t c, uint32_t r, uint32_t k
   return C::kBits == 4 ? 32u * (r % C::kF * C::kH + c / 2u) + 8u * kg + 4u * (c % 2u) : 16u * c + 4u * kg;
 }
 
+// The joint result of `own` splits of one block's `count` head-rows, by all 256
+// threads.  Each wave takes head-rows in turn for the maximum and l (lane =
+// split), then the factors of 64 splits at a time lie in LDS, and a thread adds
+// four dims of a head-row over every GR-th split, eight loads in flight.
+// AGENT: the partials come from work-groups of the same launch.
+constexpr uint32_t kMergeSplits = 64;
+struct MergeLds {
+  float factor[16][kMergeSplits];
+  float top[16], sum[16];
+  f32x4 part[256];
+};
+// Row * q_heads + head of head-row hr of a kv head.
+__device__ __forceinline__ uint32_t row_head(const ScoredArgs& a, uint32_t kv, uint32_t hr) {
+  return hr / a.group * a.q_heads + kv * a.group + hr % a.group;
+}
+template <int DIM, bool AGENT>
+__device__ __forceinline__ void merge_splits(const ScoredArgs& a, uint32_t b, uint32_t item0, uint32_t kv, uint32_t hr0,
+                                             uint32_t count, uint32_t own, MergeLds& lds) {
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
+  for (uint32_t r = wave; r < count; r += 4u) {
+    const float* ml = partial_place(a, item0, row_head(a, kv, hr0 + r)).ml;
+    const uint64_t step = uint64_t(a.rows) * a.q_heads * 2u;
+    float top = neg_inf(), sum = 0.f;
+    for (uint32_t j = lane; j < own; j += 64u) top = fmaxf(top, load_pair(ml + step * j).x);
+    top = wave_max(top);
+    for (uint32_t j = lane; j < own; j += 64u) {
+      const Pair p = load_pair(ml + step * j);
+      const float f = p.y == 0.f ? 0.f : exp_e(p.x - top);
+      sum += p.y == 0.f ? 0.f : p.y * f;
+      if (j < kMergeSplits) lds.factor[r][j] = f;
+    }
+    sum = wave_sum(sum);
+    if (lane == 0u) {
+      lds.top[r] = top;
+      lds.sum[r] = sum;
+    }
+  }
+  __syncthreads();
+  constexpr uint32_t Q = DIM / 4;
+  const uint32_t items = count * Q;                       // (head-row, four dims)
+  const uint32_t groups = items < 256u ? 256u / items : 1u;  // of splits
+  for (uint32_t base = 0; base < items; base += 256u) {
+    const uint32_t item = groups > 1u ? tid % items : base + tid, group = groups > 1u ? tid / items : 0u;
+    const bool in = item < items && group < groups;
+    const uint32_t r = in ? item / Q : 0u, quad = in ? item % Q : 0u;
+    const uint32_t local = row_head(a, kv, hr0 + r);
+    const uint64_t rh = uint64_t(b) * a.rows * a.q_heads + local, step = uint64_t(a.rows) * a.q_heads * DIM;
+    const float* o = partial_place(a, item0, local).o + 4u * quad;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    for (uint32_t c0 = 0; c0 < own; c0 += kMergeSplits) {
+      if (c0 > 0u || (base > 0u && own > kMergeSplits)) {  // the factors of these splits
+        __syncthreads();
+        for (uint32_t i = tid; i < count * kMergeSplits; i += 256u) {
+          const uint32_t rr = i / kMergeSplits, j = c0 + i % kMergeSplits;
+          if (j < own) {
+            const Pair p = load_pair(partial_place(a, item0 + j, row_head(a, kv, hr0 + rr)).ml);
+            lds.factor[rr][i % kMergeSplits] = p.y == 0.f ? 0.f : exp_e(p.x - lds.top[rr]);
+          }
+        }
+        __syncthreads();
+      }
+      const uint32_t n = own - c0 < kMergeSplits ? own - c0 : kMergeSplits;
+      if (in) {
+        for (uint32_t j0 = group; j0 < n; j0 += 8u * groups) {
+          f32x4 x[8];
+          float f[8];
+#pragma unroll
+          for (uint32_t i = 0; i < 8u; ++i) {
+            const uint32_t j = j0 + i * groups, jc = j < n ? j : j0;
+            f[i] = j < n ? lds.factor[r][jc] : 0.f;
+            const float* p = o + (c0 + jc) * step;
+            if constexpr (AGENT) {
+              const Pair lo = load_pair(p), hi = load_pair(p + 2);
+              x[i] = f32x4{lo.x, lo.y, hi.x, hi.y};
+            } else {
+              x[i] = *reinterpret_cast<const f32x4*>(p);
+            }
+          }
+#pragma unroll
+          for (uint32_t i = 0; i < 8u; ++i) {
+            if (f[i] != 0.f) acc += x[i] * f[i];  // an empty split's are not written
+          }
+        }
+      }
+    }
+    if (groups > 1u) {
+      lds.part[tid] = acc;
+      __syncthreads();
+      for (uint32_t g = 1; in && group == 0u && g < groups; ++g) acc += lds.part[g * items + item];
+    }
+    if (in && group == 0u) {
+      const float sum = lds.sum[r];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) acc[k] = sum == 0.f ? 0.f : acc[k] / sum;
+      store_out4(a, rh * a.dim + 4u * quad, acc);
+      if (quad == 0u) {
+        a.m[rh] = sum == 0.f ? neg_inf() : lds.top[r];
+        a.l[rh] = sum;
+      }
+    }
+  }
+}
+
 // LDS: Q's operands while the tiles run, then the waves' numerators, eight
-// chunks at a time (all of dim 64 and 128, half of dim 256).
+// chunks at a time (all of dim 64 and 128, half of dim 256), then the merge.
 template <class C, int QD>
 union AttendLds {
   QBlock<C, QD> q;
   f32x4 o[kAttendWaves][2 * C::kH < 8 ? 2 * C::kH : 8][64];
+  MergeLds merge;
+  __device__ AttendLds() {}
 };
 
 // Waves per SIMD that the registers allow without spills.
@@ -307,36 +424,56 @@ __global__ __launch_bounds__(64 * kAttendWaves, (kAttendOccupancy<C, ONE>)) void
   uint32_t at = blockIdx.x;
   const uint32_t kv = at % a.kv_heads;
   at /= a.kv_heads;
-  const uint32_t block = at % a.blocks;
-  at /= a.blocks;
-  const uint32_t split = at % a.splits, b = at / a.splits;
+  const uint32_t block = at % a.blocks, item = at / a.blocks;
+  WorkItem it;
+  if (!item_of(a, item, it)) return;
+  const uint32_t b = it.seq, split = it.split;
 
   const uint32_t hr = block * 16u + r / F;  // F > 1: one block
   const bool valid = hr < a.head_rows;
   const uint32_t hrc = valid ? hr : a.head_rows - 1u;
   const uint32_t row = hrc / a.group, head = kv * a.group + hrc % a.group;
-  const uint64_t rh = (uint64_t(b) * a.rows + row) * a.q_heads + head;
-  const ScoredSeq e = clamp_seq(a.seq_starts[b], a.seq_starts[b + 1u], a.page_offsets[b], a.total_tokens, a.table_entries,
-                                a.page_tokens, a.max_tokens);
+  const uint32_t local = row * a.q_heads + head;
+  const uint64_t rh = uint64_t(b) * a.rows * a.q_heads + local;
+  const ScoredSeq e = it.e;
   const int64_t qref = a.q_positions[uint64_t(b) * a.rows], qpos = a.q_positions[uint64_t(b) * a.rows + row];
-  const Visible vis = visible_tokens(a, e, b, valid, qpos);
-  const LiveTiles live = live_tiles(vis);
-  uint32_t per = live.n / a.splits + (live.n % a.splits != 0u ? 1u : 0u);
-  per = per > a.split_tiles ? per : a.split_tiles;
-  const uint32_t own = live.n > 0u ? (live.n - 1u) / per + 1u : 1u;
-  if (split >= own) {
-    if (a.splits > 1u && wave == 0u && valid && kg == 0u && r % F == 0u) {
-      float* ml = partial_place(a, rh, split).ml;
-      ml[0] = neg_inf();
-      ml[1] = 0.f;
-    }
-    return;
+  const int64_t prefix = a.prefix ? a.prefix[b] : 0;
+
+  // Everything the first K request depends on is asked for before any of it is
+  // waited for: the positions around the rows' limits, Q, and the pages of the
+  // tiles that would be this wave's if positions count up from 0 to the last
+  // row's.  That is three rounds of memory latency instead of five.
+  const Sight sight = ask_visible(a, e, qpos, prefix);
+  const auto share = [&](const LiveTiles& t) {  // least tiles of a split
+    const uint32_t per = t.n / it.count + (t.n % it.count != 0u ? 1u : 0u);
+    return per > a.split_tiles ? per : a.split_tiles;
+  };
+  const auto tile_at = [&](const LiveTiles& t, uint32_t first, uint32_t i) {
+    const uint64_t x = uint64_t(first) + uint64_t(i) * NW;
+    return t.tile(x < t.n ? uint32_t(x) : t.n - 1u);
+  };
+  const uint64_t behind = uint64_t(a.rows) - 1u + a.window;
+  const LiveTiles likely = live_tiles(prefix <= 0 ? 0u : (uint64_t(prefix) < e.tokens ? uint32_t(prefix) : e.tokens),
+                                      a.window != 0u && behind < e.tokens ? e.tokens - uint32_t(behind) : 0u, e.tokens);
+  TilePages pages{0u, 0u};
+  if (e.tokens > 0u) {
+    const uint32_t guess = split * share(likely) + wave;
+    pages = tile_pages(a, e, [&](uint32_t i) { return tile_at(likely, guess, i); }, 0u, lane);
   }
   {
     const uint32_t q_hr = block * 16u + threadIdx.x / 16u;
     const uint32_t q_row = q_hr / a.group;
     stage_q<C, QD>(a, (uint64_t(b) * a.rows + q_row) * a.q_stride + uint64_t(kv * a.group + q_hr % a.group) * a.dim,
                    q_hr < a.head_rows, lds.q);
+  }
+  const Visible vis = visible_tokens(a, e, valid, sight);
+  const LiveTiles live = live_tiles(vis.pre, vis.min_lo, vis.max_hi);
+  const uint32_t per = share(live);
+  const uint32_t own = live.n > 0u ? (live.n - 1u) / per + 1u : 1u;
+  const bool writer = wave == 0u && valid && kg == 0u && r % F == 0u;  // of m and l
+  if (split >= own) {
+    if (a.counters == nullptr && writer) store_pair(partial_place(a, item, local).ml, neg_inf(), 0.f);
+    return;
   }
   __syncthreads();
   const ScoreForm form = score_form(a, lds.q.factor[r], a.slopes ? a.slopes[head] : 0.f, near(int64_t(uint64_t(qpos) - uint64_t(qref))));
@@ -355,14 +492,12 @@ __global__ __launch_bounds__(64 * kAttendWaves, (kAttendOccupancy<C, ONE>)) void
   const uint32_t first = split * per + wave;
   const uint32_t end = live.n - split * per > per ? split * per + per : live.n;
   const uint32_t n = first < end ? (end - first + NW - 1u) / NW : 0u;
-  const auto tile_of = [&](uint32_t i) {
-    const uint64_t t = uint64_t(first) + uint64_t(i) * NW;
-    return live.tile(t < live.n ? uint32_t(t) : live.n - 1u);
-  };
+  const auto tile_of = [&](uint32_t i) { return tile_at(live, first, i); };
   uint32_t code_bits = 0x64006400u;
   asm("" : "+v"(code_bits));
   if (n > 0u) {
-    TilePages pages = tile_pages(a, e, tile_of, 0u, lane), ahead_pages = pages;
+    if (!live.same(likely)) pages = tile_pages(a, e, tile_of, 0u, lane);
+    TilePages ahead_pages = pages;
     TileRows<ONE> rows = tile_rows<ONE>(a, pages, 0u, kv);
     uint32_t t0 = tile_of(0u) * kTileTokens;
     typename C::K k = C::template load_k<ONE>(a, rows, r, kg, e.tokens - t0);
@@ -404,7 +539,7 @@ __global__ __launch_bounds__(64 * kAttendWaves, (kAttendOccupancy<C, ONE>)) void
   const float f = l == 0.f ? 0.f : to_top(s.mref2, top);  // a wave without visible tokens: 0
   if (kg == 0u) lds_l[wave][r] = l * f;
   const bool done = own == 1u;
-  const PartialPlace part = done ? PartialPlace{nullptr, nullptr} : partial_place(a, rh, split);
+  const PartialPlace part = done ? PartialPlace{nullptr, nullptr} : partial_place(a, item, local);
 #pragma unroll
   for (int round = 0; round < NC / NR; ++round) {
 #pragma unroll
@@ -432,7 +567,8 @@ __global__ __launch_bounds__(64 * kAttendWaves, (kAttendOccupancy<C, ONE>)) void
         for (int k = 0; k < 4; ++k) o[k] = sum == 0.f ? 0.f : o[k] / sum;
         store_out4(a, rh * a.dim + d, o);
       } else {
-        *reinterpret_cast<f32x4*>(part.o + d) = o;
+        store_pair(part.o + d, o[0], o[1]);
+        store_pair(part.o + d + 2, o[2], o[3]);
       }
     }
     if (round + 1 < NC / NR) __syncthreads();
@@ -440,62 +576,43 @@ __global__ __launch_bounds__(64 * kAttendWaves, (kAttendOccupancy<C, ONE>)) void
   float sum = lds_l[0][r];
 #pragma unroll
   for (int w = 1; w < NW; ++w) sum += lds_l[w][r];
-  if (wave == 0u && valid && kg == 0u && r % F == 0u) {
+  if (writer) {
     if (done) {
       a.m[rh] = sum == 0.f ? neg_inf() : top;
       a.l[rh] = sum;
-      if (a.splits > 1u) partial_place(a, rh, 0u).ml[1] = -1.f;
+      if (a.counters == nullptr) store_pair(partial_place(a, item, local).ml, top, -1.f);  // the merge passes it by
     } else {
-      part.ml[0] = top;
-      part.ml[1] = sum;
+      store_pair(part.ml, top, sum);
     }
   }
+  if (a.counters == nullptr || done) return;
+  // Every wave's partials have reached memory before the work-group's ticket is
+  // taken, so whoever draws the last ticket sees them all.
+  __shared__ uint32_t last;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  uint32_t* counter = a.counters + (uint64_t(b) * a.kv_heads + kv) * a.blocks + block;
+  if (threadIdx.x == 0u) last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1u == own;
+  __syncthreads();
+  if (last == 0u) return;
+  const uint32_t left = a.head_rows - block * 16u;
+  merge_splits<32 * C::kGroups, true>(a, b, it.first, kv, block * 16u, left < 16u ? left : 16u, own, lds.merge);
+  if (threadIdx.x == 0u) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// The joint result of a head-row's splits: one work-group of dim threads times
-// 256 / dim groups of splits per head-row.
+// The same as a second launch: a work-group per head-row.
 template <int DIM>
 __global__ __launch_bounds__(256) void scored_merge_kernel(const ScoredArgs a) {
-  constexpr int GR = 256 / (DIM / 4);  // groups of splits
-  __shared__ f32x4 lds_o[GR][DIM / 4];
-  __shared__ float lds_l[GR];
-  const uint64_t rh = blockIdx.x;
-  const PartialPlace p = partial_place(a, rh, 0u);
-  if (p.ml[1] == -1.f) return;
-  const uint32_t quad = threadIdx.x % (DIM / 4), gr = threadIdx.x / (DIM / 4), lane = threadIdx.x & 63u;
-  float top = neg_inf();
-  for (uint32_t j = lane; j < a.splits; j += 64u) top = fmaxf(top, p.ml[2u * j]);
-  top = wave_max(top);
-  f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  float l = 0.f;
-  for (uint32_t j = gr; j < a.splits; j += GR) {
-    const float lj = p.ml[2u * j + 1u];
-    if (lj == 0.f) continue;
-    const float f = exp_e(p.ml[2u * j] - top);
-    l += lj * f;
-    o += *reinterpret_cast<const f32x4*>(p.o + uint64_t(j) * DIM + 4u * quad) * f;
-  }
-  lds_o[gr][quad] = o;
-  if (quad == 0u) lds_l[gr] = l;
-  __syncthreads();
-  if (gr != 0u) return;
-#pragma unroll
-  for (int g = 1; g < GR; ++g) {
-    o += lds_o[g][quad];
-    l += lds_l[g];
-  }
-#pragma unroll
-  for (int k = 0; k < 4; ++k) o[k] = l == 0.f ? 0.f : o[k] / l;
-  store_out4(a, rh * DIM + 4u * quad, o);
-  if (quad == 0u) {
-    a.m[rh] = l == 0.f ? neg_inf() : top;
-    a.l[rh] = l;
-  }
+  __shared__ MergeLds lds;
+  const uint32_t hr = blockIdx.x % a.head_rows, item = blockIdx.x / a.head_rows, kv = item % a.kv_heads, b = item / a.kv_heads;
+  const WorkItem it = items_of(a, b);
+  if (partial_place(a, it.first, row_head(a, kv, hr)).ml[1] == -1.f) return;  // one split: written
+  merge_splits<DIM, false>(a, b, it.first, kv, hr, 1u, it.count, lds);
 }
 
 template <class C, int QD, int PD>
 inline hipError_t launch_attend_kernel(const ScoredArgs& a, hipStream_t stream) {
-  const uint32_t groups = a.batch * a.splits * a.blocks * a.kv_heads;
+  const uint32_t groups = a.items * a.blocks * a.kv_heads;
   if (a.page_tokens % kTileTokens == 0u) scored_attend_kernel<C, QD, PD, true><<<groups, 64 * kAttendWaves, 0, stream>>>(a);
   else scored_attend_kernel<C, QD, PD, false><<<groups, 64 * kAttendWaves, 0, stream>>>(a);
   return hipGetLastError();

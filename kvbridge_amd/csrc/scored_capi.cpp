@@ -163,13 +163,13 @@ int kvb_read_kv(const kvb_read_shape* s, const kvb_read_io* io, void* stream) {
 
 const char* kvb_scored_shape_error(const kvb_scored_shape* s) { return s ? kvb::scored_error(*s) : kNullShape; }
 
-int kvb_scored_split_count(const kvb_scored_shape* s, uint32_t* splits) {
-  return sized(s, splits, [](const kvb_scored_shape& x) { return kvb::scored_splits(x).splits; });
+int kvb_scored_item_count(const kvb_scored_shape* s, uint32_t* items) {
+  return sized(s, items, [](const kvb_scored_shape& x) { return kvb::scored_splits(x).items; });
 }
 
 int kvb_scored_scratch_elements(const kvb_scored_shape* s, size_t* elements) {
   return sized(s, elements, [](const kvb_scored_shape& x) {
-    return size_t(x.batch) * x.rows * x.q_heads * kvb::scored_splits(x).splits * (size_t(x.dim) + 2);
+    return size_t(kvb::scored_splits(x).items) * x.rows * x.q_heads * (size_t(x.dim) + 2);
   });
 }
 
@@ -188,10 +188,11 @@ int kvb_decode_attention_scored(const kvb_scored_shape* s, const kvb_scored_inpu
     if (off16(out) || off16(scratch)) return invalid("scratch and out must be 16-byte aligned");
     kvb::ScoredArgs a = scored_args(*s, *in);
     const kvb::ScoredSplits p = kvb::scored_splits(*s);
+    a.items = p.items;
     a.splits = p.splits;
     a.split_tiles = p.tiles;
     a.scratch = scratch;
-    a.counters = counters;
+    a.counters = kvb::scored_one_launch(*s, p) ? counters : nullptr;
     a.m = m;
     a.l = l;
     a.out = out;

@@ -16,9 +16,13 @@ const char* evict_error(const kvb_evict_shape& s);
 uint32_t scored_blocks(const kvb_scored_shape& s);  // blocks of 16 head-rows per kv head
 
 struct ScoredSplits {
-  uint32_t splits, tiles;  // partials per sequence, least tiles of a split
+  uint32_t items;   // (sequence, split) work items of a kv head and block, each with its partials
+  uint32_t splits;  // items of every sequence; 0: the kernel shares them out by the sequences' lengths
+  uint32_t tiles;   // least tiles of an item
 };
 ScoredSplits scored_splits(const kvb_scored_shape& s);
+// Whether the last work-group of a block merges its splits itself.
+bool scored_one_launch(const kvb_scored_shape& s, const ScoredSplits& p);
 
 struct ScoredChunks {
   uint32_t chunks, tiles;  // work-groups per sequence and kv head, tiles of each

@@ -53,7 +53,7 @@ __global__ __launch_bounds__(64 * kWeightWaves) void scored_weights_kernel(const
   if (c0 >= tiles) return;
   const uint32_t t_begin = uint32_t(c0), t_end = tiles - t_begin > a.chunk_tiles ? t_begin + a.chunk_tiles : tiles;
   const uint32_t fresh0 = a.fresh < e.tokens ? e.tokens - a.fresh : 0u;  // tokens from here on are set
-  const int64_t qref = a.q_positions[uint64_t(b) * a.rows];
+  const int64_t qref = a.q_positions[uint64_t(b) * a.rows], prefix = a.prefix ? a.prefix[b] : 0;
 
   for (uint32_t first = 0; first < a.blocks; first += kBlocksAtOnce<C, QD>) {
     const uint32_t count = a.blocks - first < kBlocksAtOnce<C, QD> ? a.blocks - first : kBlocksAtOnce<C, QD>;
@@ -74,7 +74,8 @@ __global__ __launch_bounds__(64 * kWeightWaves) void scored_weights_kernel(const
       const uint32_t row = hrc / a.group, head = kv * a.group + hrc % a.group;
       const uint64_t rh = (uint64_t(b) * a.rows + row) * a.q_heads + head;
       const int64_t qpos = a.q_positions[uint64_t(b) * a.rows + row];
-      const Visible vis = visible_tokens(a, e, b, valid, qpos);
+      const Visible vis = visible_tokens(a, e, valid, ask_visible(a, e, qpos, prefix));
+      pre = vis.pre;
       const float l = a.l[rh];
       const bool counts = valid && l > 0.f;
       Block& w = blocks[i];
@@ -91,11 +92,7 @@ __global__ __launch_bounds__(64 * kWeightWaves) void scored_weights_kernel(const
         w.max_hi = vis.max_hi;
       }
     }
-    if (a.prefix) {  // the prefix's end is the same for every row
-      const int64_t p = a.prefix[b];
-      if (e.tokens > 0u && p > INT64_MIN)
-        pre = uint32_t(__builtin_amdgcn_readfirstlane(int(first_above(a.k_positions + e.start, e.tokens, a.k_positions[e.start + e.tokens - 1u], p - 1))));
-    }
+    if (wave >= count && a.prefix) pre = visible_tokens(a, e, false, ask_visible(a, e, 0, prefix)).pre;  // the same for every row
     __syncthreads();
     uint32_t min_lo = 0xffffffffu, max_hi = 0u;
     for (uint32_t i = 0; i < count; ++i) {

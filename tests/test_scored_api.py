@@ -22,15 +22,18 @@ def given(**chg):
 def test_valid_shapes_and_sizes():
     s = shape()
     assert kvb.scored_shape_error(s) is None
-    n = kvb.scored_split_count(s)
-    assert 1 <= n <= 128
-    assert kvb.scored_scratch_elements(s) == 4 * 32 * n * 130
+    n = kvb.scored_item_count(s)
+    assert 4 <= n <= 4096
+    assert kvb.scored_scratch_elements(s) == n * 32 * 130
     assert kvb.scored_counter_elements(s) == 4 * 8
     assert kvb.scored_counter_elements(s.copy(rows=5)) == 4 * 8 * 2  # 20 head-rows: two blocks of 16
-    assert kvb.scored_split_count(shape(split_tokens=2048)) == 64
-    assert kvb.scored_split_count(shape(max_tokens=1)) == 1
+    # with a split size: every sequence the splits of max_tokens
+    assert kvb.scored_item_count(shape(split_tokens=2048)) == 4 * 64
+    assert kvb.scored_item_count(shape(max_tokens=1)) == 4
     # a window bounds the tokens that are cut
-    assert kvb.scored_split_count(shape(split_tokens=512, window=1000)) == -(-(1000 + 1 + 32 + 31) // 32 // 16)
+    assert kvb.scored_item_count(shape(split_tokens=512, window=1000)) == 4 * -(-(1000 + 1 + 32 + 31) // 32 // 16)
+    # more sequences than the kernel shares items out for
+    assert kvb.scored_item_count(shape(batch=300, max_tokens=4000)) >= 300
 
 
 @pytest.mark.parametrize("change,msg", [
@@ -63,7 +66,7 @@ def test_valid_shapes_and_sizes():
 def test_scored_rejections_in_order(change, msg):
     s = shape(**change)
     assert kvb.scored_shape_error(s) == msg
-    for f in (kvb.scored_split_count, kvb.scored_scratch_elements, kvb.scored_counter_elements):
+    for f in (kvb.scored_item_count, kvb.scored_scratch_elements, kvb.scored_counter_elements):
         with pytest.raises(kvb.KvbInvalidArgument) as e:
             f(s)
         assert str(e.value) == msg
