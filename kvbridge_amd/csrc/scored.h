@@ -634,22 +634,23 @@ struct QBlock {
   float factor[16];                                // score = factor * (sum of the scaled products)
 };
 
-// By all 256 threads: thread 16 r + s takes 2 G dims from 2 G s of head-row r,
-// so that the maximum over a row is one over 16 lanes.  `at`: element index
-// of the head-row's Q.  The caller's barrier follows.
+// With F > 1 the operands are cleared first, by n threads; a barrier follows.
 template <class C, int QD>
-__device__ __forceinline__ void stage_q(const ScoredArgs& a, uint64_t at, bool valid, QBlock<C, QD>& q) {
+__device__ __forceinline__ void clear_q(QBlock<C, QD>& q, uint32_t tid, uint32_t n) {
+  if constexpr (C::kF > 1) {
+    const f16x8 zero = {0, 0, 0, 0, 0, 0, 0, 0};
+    for (uint32_t i = tid; i < uint32_t(C::kGroups * QD * 64); i += n) (&q.d[0][0][0])[i] = zero;
+  }
+}
+// By 256 threads (four whole waves): thread 16 r + s takes 2 G dims from 2 G s
+// of head-row r, so that the maximum over a row is one over 16 lanes.  `at`:
+// element index of the head-row's Q.  The caller's barrier follows.
+template <class C, int QD>
+__device__ __forceinline__ void stage_q(const ScoredArgs& a, uint64_t at, bool valid, QBlock<C, QD>& q, uint32_t tid) {
   constexpr int G = C::kGroups, N = 2 * G;
   constexpr int F = C::kF, H = C::kH;
-  const uint32_t r = threadIdx.x / 16u, s = threadIdx.x % 16u, d0 = s * N;
-  if constexpr (F > 1) {
-    const f16x8 zero = {0, 0, 0, 0, 0, 0, 0, 0};
-    f16x8* all = &q.d[0][0][0];
-#pragma unroll
-    for (int i = 0; i < G * QD / 4; ++i) all[i * 256 + threadIdx.x] = zero;
-    __syncthreads();
-    if (r >= 16u / F) return;
-  }
+  const uint32_t r = tid / 16u, s = tid % 16u, d0 = s * N;
+  if (r >= 16u / F) return;
   float x[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) x[i] = 0.f;

@@ -1,8 +1,12 @@
 // Ragged decode attention over a 4- or 8-bit cache under score forms
 // (kvb_decode_attention_scored): the split kernel.
 //
-// A work-group of four waves takes one split of (sequence, kv head, block of 16
-// head-rows); its waves take every fourth 32-token tile.  One pass over the
+// A work-group takes one split of (sequence, kv head, block of 16 head-rows), its
+// waves the split's 32-token tiles in turn.  It has all the waves that a CU
+// holds of this kernel (12 or 8: few partials, which it can merge itself) where
+// the sequences are few, and 4 where they are many and finer parts balance
+// better: 16 ragged sequences 78 us against 85, one of 64K tokens 27.7 against
+// 27.0 (scored_splits in scored_shape.cpp).  One pass over the
 // tokens with a running reference mref per head-row (not the maximum itself:
 // it moves only when a score exceeds it by 5.5, so that most tiles rescale
 // nothing), l in fp32, and the output's numerators in MFMA
@@ -18,8 +22,6 @@
 #include "scored.h"
 
 namespace kvb {
-
-constexpr int kAttendWaves = 4;
 
 // Partials of item w: (max score, l) pairs of its head-rows, then the
 // numerators: scratch[(w * row_heads + rh) * 2], scratch[2 * items * row_heads +
@@ -297,7 +299,7 @@ __device__ __forceinline__ uint32_t chunk_dim(uint32_t c, uint32_t r, uint32_t k
   return C::kBits == 4 ? 32u * (r % C::kF * C::kH + c / 2u) + 8u * kg + 4u * (c % 2u) : 16u * c + 4u * kg;
 }
 
-// The joint result of `own` splits of one block's `count` head-rows, by all 256
+// The joint result of `own` splits of one block's `count` head-rows, by NT
 // threads.  Each wave takes head-rows in turn for the maximum and l (lane =
 // split), then the factors of 64 splits at a time lie in LDS, and a thread adds
 // four dims of a head-row over every GR-th split, eight loads in flight.
@@ -306,7 +308,7 @@ constexpr uint32_t kMergeSplits = 64;
 struct MergeLds {
   float factor[16][kMergeSplits];
   float top[16], sum[16];
-  f32x4 part[256];
+  f32x4 part[1];  // NT
 };
 // Row * q_heads + head of head-row hr of a kv head.
 __device__ __forceinline__ uint32_t row_head(const ScoredArgs& a, uint32_t kv, uint32_t hr) {
@@ -314,9 +316,9 @@ __device__ __forceinline__ uint32_t row_head(const ScoredArgs& a, uint32_t kv, u
 }
 template <int DIM, bool AGENT>
 __device__ __forceinline__ void merge_splits(const ScoredArgs& a, uint32_t b, uint32_t item0, uint32_t kv, uint32_t hr0,
-                                             uint32_t count, uint32_t own, MergeLds& lds) {
+                                             uint32_t count, uint32_t own, MergeLds& lds, uint32_t NT) {
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
-  for (uint32_t r = wave; r < count; r += 4u) {
+  for (uint32_t r = wave; r < count; r += NT / 64u) {
     const float* ml = partial_place(a, item0, row_head(a, kv, hr0 + r)).ml;
     const uint64_t step = uint64_t(a.rows) * a.q_heads * 2u;
     float top = neg_inf(), sum = 0.f;
@@ -337,8 +339,8 @@ __device__ __forceinline__ void merge_splits(const ScoredArgs& a, uint32_t b, ui
   __syncthreads();
   constexpr uint32_t Q = DIM / 4;
   const uint32_t items = count * Q;                       // (head-row, four dims)
-  const uint32_t groups = items < 256u ? 256u / items : 1u;  // of splits
-  for (uint32_t base = 0; base < items; base += 256u) {
+  const uint32_t groups = items < NT ? NT / items : 1u;  // of splits
+  for (uint32_t base = 0; base < items; base += NT) {
     const uint32_t item = groups > 1u ? tid % items : base + tid, group = groups > 1u ? tid / items : 0u;
     const bool in = item < items && group < groups;
     const uint32_t r = in ? item / Q : 0u, quad = in ? item % Q : 0u;
@@ -349,7 +351,7 @@ __device__ __forceinline__ void merge_splits(const ScoredArgs& a, uint32_t b, ui
     for (uint32_t c0 = 0; c0 < own; c0 += kMergeSplits) {
       if (c0 > 0u || (base > 0u && own > kMergeSplits)) {  // the factors of these splits
         __syncthreads();
-        for (uint32_t i = tid; i < count * kMergeSplits; i += 256u) {
+        for (uint32_t i = tid; i < count * kMergeSplits; i += NT) {
           const uint32_t rr = i / kMergeSplits, j = c0 + i % kMergeSplits;
           if (j < own) {
             const Pair p = load_pair(partial_place(a, item0 + j, row_head(a, kv, hr0 + rr)).ml);
@@ -400,51 +402,78 @@ __device__ __forceinline__ void merge_splits(const ScoredArgs& a, uint32_t b, ui
   }
 }
 
-// LDS: Q's operands while the tiles run, then the waves' numerators, eight
-// chunks at a time (all of dim 64 and 128, half of dim 256), then the merge.
+// LDS of a work-group of `waves`: Q's operands while the tiles run, then the
+// waves' numerators, up to eight chunks at a time, then the merge.
+template <class C>
+constexpr int kChunksAtOnce = 2 * C::kH < 8 ? 2 * C::kH : 8;
 template <class C, int QD>
-union AttendLds {
-  QBlock<C, QD> q;
-  f32x4 o[kAttendWaves][2 * C::kH < 8 ? 2 * C::kH : 8][64];
-  MergeLds merge;
-  __device__ AttendLds() {}
+constexpr uint32_t attend_lds(uint32_t waves) {
+  const uint32_t q = sizeof(QBlock<C, QD>), o = waves * kChunksAtOnce<C> * 64u * 16u, m = sizeof(MergeLds) + waves * 64u * 16u;
+  return q > o ? (q > m ? q : m) : (o > m ? o : m);
+}
+
+// What the first wave finds out for the work-group: its item and the columns'
+// visible tokens.
+struct AttendPlan {
+  WorkItem it;
+  uint32_t found, pre, min_lo, max_hi, all_lo, all_hi;
+  uint32_t lo[16], hi[16];
+  float slope[16];
+  int back[16];
+  int64_t qref;
 };
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return uint32_t(__builtin_amdgcn_readfirstlane(int(x))); }
 
 // Waves per SIMD that the registers allow without spills.
 template <class C, bool ONE>
 constexpr int kAttendOccupancy = C::kGroups == 8 || (C::kF > 1 && C::kH > 1) || (C::kBits == 8 && !ONE) ? 2 : 3;
 
 template <class C, int QD, int PD, bool ONE>
-__global__ __launch_bounds__(64 * kAttendWaves, (kAttendOccupancy<C, ONE>)) void scored_attend_kernel(const ScoredArgs a) {
-  constexpr int F = C::kF, NC = 2 * C::kH, NW = kAttendWaves, NR = NC < 8 ? NC : 8;
-  __shared__ AttendLds<C, QD> lds;
-  __shared__ float lds_m[NW][16], lds_l[NW][16];
+__global__ __launch_bounds__((256 * kAttendOccupancy<C, ONE>), (kAttendOccupancy<C, ONE>)) void scored_attend_kernel(const ScoredArgs a) {
+  constexpr int F = C::kF, NC = 2 * C::kH, NR = kChunksAtOnce<C>, MW = 4 * kAttendOccupancy<C, ONE>;
+  extern __shared__ __align__(16) uint8_t lds_raw[];
+  QBlock<C, QD>& lds_q = *reinterpret_cast<QBlock<C, QD>*>(lds_raw);
+  f32x4(*const lds_o)[NR][64] = reinterpret_cast<f32x4(*)[NR][64]>(lds_raw);  // [wave]
+  __shared__ AttendPlan plan;
+  __shared__ float lds_m[MW][16], lds_l[MW][16];
+  const uint32_t NW = blockDim.x >> 6;
   const uint32_t lane = threadIdx.x & 63u, r = lane & 15u, kg = lane >> 4;
-  const uint32_t wave = uint32_t(__builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6)));
-  uint32_t at = blockIdx.x;
-  const uint32_t kv = at % a.kv_heads;
-  at /= a.kv_heads;
+  const uint32_t wave = uniform(threadIdx.x >> 6);
+  const uint32_t kv = blockIdx.x % a.kv_heads, at = blockIdx.x / a.kv_heads;
   const uint32_t block = at % a.blocks, item = at / a.blocks;
-  WorkItem it;
-  if (!item_of(a, item, it)) return;
-  const uint32_t b = it.seq, split = it.split;
-
   const uint32_t hr = block * 16u + r / F;  // F > 1: one block
   const bool valid = hr < a.head_rows;
   const uint32_t hrc = valid ? hr : a.head_rows - 1u;
   const uint32_t row = hrc / a.group, head = kv * a.group + hrc % a.group;
+
+  // The first wave finds the item; everybody clears Q's operands meanwhile.
+  if (wave == 0u) {
+    WorkItem w{0u, 0u, 0u, 0u, ScoredSeq{0u, 0u, 0u}};
+    const bool found = item_of(a, item, w);
+    if (lane == 0u) {
+      plan.it = w;
+      plan.found = found ? 1u : 0u;
+    }
+  }
+  clear_q(lds_q, threadIdx.x, 64u * NW);
+  __syncthreads();
+  if (uniform(plan.found) == 0u) return;
+  WorkItem it;
+  it.seq = uniform(plan.it.seq);
+  it.split = uniform(plan.it.split);
+  it.count = uniform(plan.it.count);
+  it.first = uniform(plan.it.first);
+  it.e = ScoredSeq{uniform(plan.it.e.start), uniform(plan.it.e.tokens), uniform(plan.it.e.table_off)};
+  const uint32_t b = it.seq, split = it.split;
   const uint32_t local = row * a.q_heads + head;
   const uint64_t rh = uint64_t(b) * a.rows * a.q_heads + local;
   const ScoredSeq e = it.e;
-  const int64_t qref = a.q_positions[uint64_t(b) * a.rows], qpos = a.q_positions[uint64_t(b) * a.rows + row];
-  const int64_t prefix = a.prefix ? a.prefix[b] : 0;
 
   // Everything the first K request depends on is asked for before any of it is
-  // waited for: the positions around the rows' limits, Q, and the pages of the
-  // tiles that would be this wave's if positions count up from 0 to the last
-  // row's.  That is three rounds of memory latency instead of five.
-  const Sight sight = ask_visible(a, e, qpos, prefix);
-  const auto share = [&](const LiveTiles& t) {  // least tiles of a split
+  // waited for: by the first wave the positions around the rows' limits, by the
+  // next four Q, and by all the pages of the tiles that would be theirs if
+  // positions count up from 0 to the last row's.
+  const auto share = [&](const LiveTiles& t) {  // tiles of a split
     const uint32_t per = t.n / it.count + (t.n % it.count != 0u ? 1u : 0u);
     return per > a.split_tiles ? per : a.split_tiles;
   };
@@ -452,6 +481,7 @@ __global__ __launch_bounds__(64 * kAttendWaves, (kAttendOccupancy<C, ONE>)) void
     const uint64_t x = uint64_t(first) + uint64_t(i) * NW;
     return t.tile(x < t.n ? uint32_t(x) : t.n - 1u);
   };
+  const int64_t prefix = a.prefix ? a.prefix[b] : 0;
   const uint64_t behind = uint64_t(a.rows) - 1u + a.window;
   const LiveTiles likely = live_tiles(prefix <= 0 ? 0u : (uint64_t(prefix) < e.tokens ? uint32_t(prefix) : e.tokens),
                                       a.window != 0u && behind < e.tokens ? e.tokens - uint32_t(behind) : 0u, e.tokens);
@@ -460,13 +490,34 @@ __global__ __launch_bounds__(64 * kAttendWaves, (kAttendOccupancy<C, ONE>)) void
     const uint32_t guess = split * share(likely) + wave;
     pages = tile_pages(a, e, [&](uint32_t i) { return tile_at(likely, guess, i); }, 0u, lane);
   }
-  {
-    const uint32_t q_hr = block * 16u + threadIdx.x / 16u;
-    const uint32_t q_row = q_hr / a.group;
-    stage_q<C, QD>(a, (uint64_t(b) * a.rows + q_row) * a.q_stride + uint64_t(kv * a.group + q_hr % a.group) * a.dim,
-                   q_hr < a.head_rows, lds.q);
+  if (wave == 0u) {
+    const int64_t qref = a.q_positions[uint64_t(b) * a.rows], qpos = a.q_positions[uint64_t(b) * a.rows + row];
+    const Visible v = visible_tokens(a, e, valid, ask_visible(a, e, qpos, prefix));
+    if (kg == 0u) {
+      plan.lo[r] = v.lo;
+      plan.hi[r] = v.hi;
+      plan.slope[r] = a.slopes ? a.slopes[head] : 0.f;
+      plan.back[r] = near(int64_t(uint64_t(qpos) - uint64_t(qref)));
+    }
+    if (lane == 0u) {
+      plan.pre = v.pre;
+      plan.min_lo = v.min_lo;
+      plan.max_hi = v.max_hi;
+      plan.all_lo = v.all_lo;
+      plan.all_hi = v.all_hi;
+      plan.qref = qref;
+    }
   }
-  const Visible vis = visible_tokens(a, e, valid, sight);
+  const uint32_t stager = NW > 4u ? wave - 1u : wave;  // four waves for Q, not the first where there are more
+  if (stager < 4u) {
+    const uint32_t tid = stager * 64u + lane, q_hr = block * 16u + tid / 16u;
+    stage_q<C, QD>(a, (uint64_t(b) * a.rows + q_hr / a.group) * a.q_stride + uint64_t(kv * a.group + q_hr % a.group) * a.dim,
+                   q_hr < a.head_rows, lds_q, tid);
+  }
+  __syncthreads();
+  const Visible vis{plan.lo[r], plan.hi[r], uniform(plan.pre), uniform(plan.min_lo), uniform(plan.max_hi), uniform(plan.all_lo),
+                    uniform(plan.all_hi)};
+  const int64_t qref = plan.qref;
   const LiveTiles live = live_tiles(vis.pre, vis.min_lo, vis.max_hi);
   const uint32_t per = share(live);
   const uint32_t own = live.n > 0u ? (live.n - 1u) / per + 1u : 1u;
@@ -475,8 +526,7 @@ __global__ __launch_bounds__(64 * kAttendWaves, (kAttendOccupancy<C, ONE>)) void
     if (a.counters == nullptr && writer) store_pair(partial_place(a, item, local).ml, neg_inf(), 0.f);
     return;
   }
-  __syncthreads();
-  const ScoreForm form = score_form(a, lds.q.factor[r], a.slopes ? a.slopes[head] : 0.f, near(int64_t(uint64_t(qpos) - uint64_t(qref))));
+  const ScoreForm form = score_form(a, lds_q.factor[r], plan.slope[r], plan.back[r]);
 
   AttendState<C> s;
 #pragma unroll
@@ -512,7 +562,7 @@ __global__ __launch_bounds__(64 * kAttendWaves, (kAttendOccupancy<C, ONE>)) void
       const int ahead_next = load_ahead<C>(a, e, t_next, r, kg, qref);
       asm volatile("" ::: "memory");  // Q's operands stay in LDS: not hoisted out of the loop
       float x[8];
-      tile_scores<C, QD>(k, lds.q, lane, x);
+      tile_scores<C, QD>(k, lds_q, lane, x);
       const bool whole = t0 + kTileTokens <= vis.pre || (t0 >= vis.all_lo && t0 + kTileTokens <= vis.all_hi);
       apply_form<C>(a, form, ahead, t0, kg, !whole, vis.lo, vis.hi, vis.pre, x);
       s.mtop = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])), s.mtop));
@@ -526,7 +576,7 @@ __global__ __launch_bounds__(64 * kAttendWaves, (kAttendOccupancy<C, ONE>)) void
     }
   }
 
-  // The waves' parts: a common maximum, then each wave adds a quarter of the dims.
+  // The waves' parts: a common maximum, then each chunk of dims is added by one wave.
   const float l = rows_sum(s.l), mtop = rows_max(s.mtop);
   if (kg == 0u) lds_m[wave][r] = mtop;
   float mid[C::kBits == 4 ? C::kH : 1];
@@ -534,8 +584,7 @@ __global__ __launch_bounds__(64 * kAttendWaves, (kAttendOccupancy<C, ONE>)) void
   for (int h = 0; h < (C::kBits == 4 ? C::kH : 1); ++h) mid[h] = rows_sum(s.mid[h]);
   __syncthreads();  // also: every wave is done with Q
   float top = lds_m[0][r];
-#pragma unroll
-  for (int w = 1; w < NW; ++w) top = fmaxf(top, lds_m[w][r]);
+  for (uint32_t w = 1; w < NW; ++w) top = fmaxf(top, lds_m[w][r]);
   const float f = l == 0.f ? 0.f : to_top(s.mref2, top);  // a wave without visible tokens: 0
   if (kg == 0u) lds_l[wave][r] = l * f;
   const bool done = own == 1u;
@@ -547,17 +596,16 @@ __global__ __launch_bounds__(64 * kAttendWaves, (kAttendOccupancy<C, ONE>)) void
       f32x4 o = chunk_value(s, round * NR + c, mid, r);
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[i] = l == 0.f ? 0.f : o[i] * f;
-      lds.o[wave][c][lane] = o;
+      lds_o[wave][c][lane] = o;
     }
     __syncthreads();
-    // Wave w: chunks w, w + 4 (a wave's lanes are the tiles' lanes again).
-#pragma unroll
+    // A chunk to a wave (its lanes are the tiles' lanes again).
     for (uint32_t c = wave; c < uint32_t(NR); c += NW) {
-      f32x4 o = lds.o[0][c][lane];
+      f32x4 o = lds_o[0][c][lane];
       float sum = lds_l[0][r];
-#pragma unroll
-      for (int w = 1; w < NW; ++w) {
-        o += lds.o[w][c][lane];
+#pragma unroll 4
+      for (uint32_t w = 1; w < NW; ++w) {
+        o += lds_o[w][c][lane];
         sum += lds_l[w][r];
       }
       if (!valid) continue;
@@ -574,8 +622,7 @@ __global__ __launch_bounds__(64 * kAttendWaves, (kAttendOccupancy<C, ONE>)) void
     if (round + 1 < NC / NR) __syncthreads();
   }
   float sum = lds_l[0][r];
-#pragma unroll
-  for (int w = 1; w < NW; ++w) sum += lds_l[w][r];
+  for (uint32_t w = 1; w < NW; ++w) sum += lds_l[w][r];
   if (writer) {
     if (done) {
       a.m[rh] = sum == 0.f ? neg_inf() : top;
@@ -596,25 +643,36 @@ __global__ __launch_bounds__(64 * kAttendWaves, (kAttendOccupancy<C, ONE>)) void
   __syncthreads();
   if (last == 0u) return;
   const uint32_t left = a.head_rows - block * 16u;
-  merge_splits<32 * C::kGroups, true>(a, b, it.first, kv, block * 16u, left < 16u ? left : 16u, own, lds.merge);
+  merge_splits<32 * C::kGroups, true>(a, b, it.first, kv, block * 16u, left < 16u ? left : 16u, own,
+                                      *reinterpret_cast<MergeLds*>(lds_raw), 64u * NW);
   if (threadIdx.x == 0u) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
 // The same as a second launch: a work-group per head-row.
 template <int DIM>
 __global__ __launch_bounds__(256) void scored_merge_kernel(const ScoredArgs a) {
-  __shared__ MergeLds lds;
+  extern __shared__ __align__(16) uint8_t lds_raw[];
   const uint32_t hr = blockIdx.x % a.head_rows, item = blockIdx.x / a.head_rows, kv = item % a.kv_heads, b = item / a.kv_heads;
   const WorkItem it = items_of(a, b);
   if (partial_place(a, it.first, row_head(a, kv, hr)).ml[1] == -1.f) return;  // one split: written
-  merge_splits<DIM, false>(a, b, it.first, kv, hr, 1u, it.count, lds);
+  merge_splits<DIM, false>(a, b, it.first, kv, hr, 1u, it.count, *reinterpret_cast<MergeLds*>(lds_raw), 256u);
 }
 
 template <class C, int QD, int PD>
 inline hipError_t launch_attend_kernel(const ScoredArgs& a, hipStream_t stream) {
   const uint32_t groups = a.items * a.blocks * a.kv_heads;
-  if (a.page_tokens % kTileTokens == 0u) scored_attend_kernel<C, QD, PD, true><<<groups, 64 * kAttendWaves, 0, stream>>>(a);
-  else scored_attend_kernel<C, QD, PD, false><<<groups, 64 * kAttendWaves, 0, stream>>>(a);
+  const bool one = a.page_tokens % kTileTokens == 0u;
+  const uint32_t most = 4u * uint32_t(one ? kAttendOccupancy<C, true> : kAttendOccupancy<C, false>);
+  const uint32_t waves = a.waves < most ? a.waves : most, bytes = attend_lds<C, QD>(waves);
+  // LDS past 64 KiB has to be asked for.
+  if (bytes > 65536u) {
+    const hipError_t e = hipFuncSetAttribute(one ? reinterpret_cast<const void*>(scored_attend_kernel<C, QD, PD, true>)
+                                                 : reinterpret_cast<const void*>(scored_attend_kernel<C, QD, PD, false>),
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
+    if (e != hipSuccess) return e;
+  }
+  if (one) scored_attend_kernel<C, QD, PD, true><<<groups, 64u * waves, bytes, stream>>>(a);
+  else scored_attend_kernel<C, QD, PD, false><<<groups, 64u * waves, bytes, stream>>>(a);
   return hipGetLastError();
 }
 // Weights of one digit only where the output is bf16 and q has 16 bits.

@@ -13,9 +13,9 @@ hipError_t launch_scored_attend(const ScoredArgs& a, hipStream_t stream) {
     e = a.dim == 64u ? launch_attend8_d64(a, stream) : a.dim == 128u ? launch_attend8_d128(a, stream) : launch_attend8_d256(a, stream);
   if (e != hipSuccess || a.items == a.batch || a.counters) return e;  // an item each: nothing to merge
   const uint32_t groups = a.batch * a.kv_heads * a.head_rows;
-  if (a.dim == 64u) scored_merge_kernel<64><<<groups, 256, 0, stream>>>(a);
-  else if (a.dim == 128u) scored_merge_kernel<128><<<groups, 256, 0, stream>>>(a);
-  else scored_merge_kernel<256><<<groups, 256, 0, stream>>>(a);
+  if (a.dim == 64u) scored_merge_kernel<64><<<groups, 256, sizeof(MergeLds) + 256u * 16u, stream>>>(a);
+  else if (a.dim == 128u) scored_merge_kernel<128><<<groups, 256, sizeof(MergeLds) + 256u * 16u, stream>>>(a);
+  else scored_merge_kernel<256><<<groups, 256, sizeof(MergeLds) + 256u * 16u, stream>>>(a);
   return hipGetLastError();
 }
 

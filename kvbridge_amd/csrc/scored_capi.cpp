@@ -191,6 +191,7 @@ int kvb_decode_attention_scored(const kvb_scored_shape* s, const kvb_scored_inpu
     a.items = p.items;
     a.splits = p.splits;
     a.split_tiles = p.tiles;
+    a.waves = p.waves;
     a.scratch = scratch;
     a.counters = kvb::scored_one_launch(*s, p) ? counters : nullptr;
     a.m = m;

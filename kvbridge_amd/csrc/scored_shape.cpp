@@ -46,46 +46,53 @@ uint32_t scored_blocks(const kvb_scored_shape& s) { return ceil_div(uint64_t(s.r
 
 namespace {
 
-// Work-groups of the attention kernel that 256 CUs hold at once (its registers:
-// kAttendOccupancy in scored_attend.h).
-uint64_t resident_groups(const kvb_scored_shape& s) {
+constexpr uint64_t kCus = 256;
+
+// Waves of the attention kernel that a CU holds (kAttendOccupancy in
+// scored_attend.h).
+uint32_t resident_waves(const kvb_scored_shape& s) {
   const uint64_t head_rows = uint64_t(s.rows) * (s.q_heads / s.kv_heads), blocks = s.dim / 32;
   const bool half = s.kv_bits == 4 && s.dim > 64 && head_rows > 16 / blocks && head_rows <= 32 / blocks;
-  return 256 * (s.dim == 256 || half ? 2 : 3);
+  return s.dim == 256 || half || (s.kv_bits == 8 && s.page_tokens % 32 != 0) ? 8 : 12;
 }
 
 }  // namespace
 
 // Work items.  Where the caller names no split size, there are as many as fit
 // the GPU at once and the kernel shares them out over the sequences by length
-// (scored.h, item_of): every work-group then has the same number of tiles and
-// pays for its start and end once.
+// (scored.h, item_of): every work-group then has about the same number of tiles
+// and pays for its start and end once.  An item is a whole CU's unless the
+// sequences are so many that rounding to whole items would idle over a
+// sixteenth of them; then work-groups have four waves.
 ScoredSplits scored_splits(const kvb_scored_shape& s) {
   const uint64_t seen = s.window == 0 ? s.max_tokens
                                       : std::min<uint64_t>(s.max_tokens, uint64_t(s.window) + s.rows + 32);
   const uint64_t tiles = (seen + 31) / 32, others = uint64_t(s.kv_heads) * scored_blocks(s);
+  const uint32_t all = resident_waves(s);
+  const uint32_t waves = s.batch * 8 <= std::max<uint64_t>(8, kCus / others) ? all : 4;
+  const uint64_t resident = kCus * (all / waves);
   if (s.split_tokens != 0 || s.batch > 256) {
     uint64_t per = s.split_tokens / 32;
     if (per == 0) {
-      const uint64_t splits = std::max<uint64_t>(1, resident_groups(s) * 2 / (others * s.batch));
+      const uint64_t splits = std::max<uint64_t>(1, resident * 2 / (others * s.batch));
       per = std::max<uint64_t>(16, (tiles + splits - 1) / splits);
     }
     const uint64_t splits = std::max<uint64_t>(1, (tiles + per - 1) / per);
     return ScoredSplits{uint32_t(std::min<uint64_t>(s.batch * splits, 0xffffffffu)), uint32_t(std::min<uint64_t>(splits, 0xffffffffu)),
-                        uint32_t(per)};
+                        uint32_t(per), per < all ? 4u : waves};
   }
   const uint64_t least = 16, useful = s.batch * ((tiles + least - 1) / least);
-  const uint64_t items = std::max<uint64_t>(s.batch, std::min(useful, resident_groups(s) / others));
-  return ScoredSplits{uint32_t(items), s.batch == 1 ? uint32_t(items) : 0, uint32_t(least)};
+  const uint64_t items = std::max<uint64_t>(s.batch, std::min(useful, resident / others));
+  return ScoredSplits{uint32_t(items), s.batch == 1 ? uint32_t(items) : 0, uint32_t(least), waves};
 }
 
 // One work-group's merge reads the partials of up to 16 head-rows past its L2,
-// eight splits a round: with 128 splits of 4 head-rows that took 14 us, a
-// second launch over all head-rows 5.
+// eight splits of a thread's four dims a round: at most four rounds.  With 128
+// splits of 4 head-rows by 256 threads that took 14 us, a second launch over all
+// head-rows 5.
 bool scored_one_launch(const kvb_scored_shape& s, const ScoredSplits& p) {
   const uint64_t head_rows = std::min<uint64_t>(16, uint64_t(s.rows) * (s.q_heads / s.kv_heads));
-  const uint64_t rounds = (head_rows * s.dim / 4 + 255) / 256, splits = p.items / s.batch;
-  return splits * rounds <= 24;
+  return p.items / s.batch * head_rows * (s.dim / 4) <= 32 * 64 * p.waves;
 }
 
 const char* scored_error(const kvb_scored_shape& s) {

@@ -19,6 +19,7 @@ struct ScoredSplits {
   uint32_t items;   // (sequence, split) work items of a kv head and block, each with its partials
   uint32_t splits;  // items of every sequence; 0: the kernel shares them out by the sequences' lengths
   uint32_t tiles;   // least tiles of an item
+  uint32_t waves;   // of a work-group
 };
 ScoredSplits scored_splits(const kvb_scored_shape& s);
 // Whether the last work-group of a block merges its splits itself.

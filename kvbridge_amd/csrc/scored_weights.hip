@@ -61,10 +61,12 @@ __global__ __launch_bounds__(64 * kWeightWaves) void scored_weights_kernel(const
       __threadfence();  // what the first pass set is in place before it is added to
       __syncthreads();  // and every wave is done with the last pass's operands
     }
+    for (uint32_t i = 0; i < count; ++i) clear_q(blocks[i].q, threadIdx.x, 64u * kWeightWaves);
+    if (C::kF > 1) __syncthreads();
     for (uint32_t i = 0; i < count; ++i) {
       const uint32_t hr = (first + i) * 16u + threadIdx.x / 16u;
       stage_q<C, QD>(a, (uint64_t(b) * a.rows + hr / a.group) * a.q_stride + uint64_t(kv * a.group + hr % a.group) * a.dim,
-                     hr < a.head_rows, blocks[i].q);
+                     hr < a.head_rows, blocks[i].q, threadIdx.x);
     }
     uint32_t pre = 0;
     for (uint32_t i = wave; i < count; i += kWeightWaves) {
