@@ -4,9 +4,9 @@
 // uint32 of its weight (the kv heads summed in fp64, rounded to fp32; always-
 // kept tokens the largest key, NaN the least).  evict_pick_kernel, one
 // work-group per sequence, finds the key of rank n by three radix passes of 11,
-// 11 and 10 bits over LDS histograms, then lets every wave run over its share
-// of the tokens in order: above the key they stay, of those equal to it the
-// first ones.
+// 11 and 10 bits over LDS histograms (four copies: most keys share few leading
+// digits), the keys of up to 32K tokens staying in registers, then writes the
+// tokens in order: above the key they stay, of those equal to it the first ones.
 // Move: one work-group per 64 kept tokens and kv head copies rows in 16-byte
 // pieces (int8 V, dim-major, byte by byte gathered to dwords).
 #include "device_common.h"
@@ -17,7 +17,7 @@ namespace {
 
 typedef uint32_t u32x4_e __attribute__((ext_vector_type(4)));
 
-constexpr uint32_t kPickThreads = 1024, kPickWaves = kPickThreads / 64, kBins = 2048;
+constexpr uint32_t kPickThreads = 1024, kPickWaves = kPickThreads / 64, kBins = 2048, kCopies = 4;
 
 __device__ __forceinline__ ScoredSeq evict_seq(const EvictArgs& a, uint32_t b) {
   return clamp_seq(a.seq_starts[b], a.seq_starts[b + 1u], a.page_offsets[b], a.total_tokens, a.table_entries, a.page_tokens,
@@ -27,7 +27,7 @@ __device__ __forceinline__ ScoredSeq evict_seq(const EvictArgs& a, uint32_t b) {
 __global__ __launch_bounds__(256) void evict_keys_kernel(const EvictArgs a) {
   const uint32_t b = blockIdx.y, t = blockIdx.x * 256u + threadIdx.x;
   const ScoredSeq e = evict_seq(a, b);
-  if (t >= e.tokens) return;
+  if (t >= e.tokens || e.tokens <= a.keep) return;  // all stay: no key is looked at
   uint32_t key = 0xffffffffu;
   if (t >= a.sink && e.tokens - t > a.recent) {
     const uint32_t lp = t / a.page_tokens, slot = t - lp * a.page_tokens;
@@ -35,19 +35,51 @@ __global__ __launch_bounds__(256) void evict_keys_kernel(const EvictArgs a) {
     page = page < a.pages ? page : a.pages - 1u;
     const float* w = a.weights_in + uint64_t(page) * a.kv_heads * a.page_tokens + slot;
     double sum = 0.0;
-    for (uint32_t h = 0; h < a.kv_heads; ++h) sum += double(w[uint64_t(h) * a.page_tokens]);
+    for (uint32_t h0 = 0; h0 < a.kv_heads; h0 += 8u) {  // eight heads' loads at once
+      float x[8];
+#pragma unroll
+      for (uint32_t i = 0; i < 8u; ++i) x[i] = h0 + i < a.kv_heads ? w[uint64_t(h0 + i) * a.page_tokens] : 0.f;
+#pragma unroll
+      for (uint32_t i = 0; i < 8u; ++i) sum += h0 + i < a.kv_heads ? double(x[i]) : 0.0;
+    }
     const float f = float(sum) + 0.f;  // -0 becomes 0
     const uint32_t u = __float_as_uint(f);
     key = f != f ? 0u : ((u >> 31) != 0u ? ~u : u | 0x80000000u);
   }
-  a.scratch[uint64_t(b) * a.max_tokens + t] = key;
+  a.scratch[uint64_t(b) * a.scratch_stride + t] = key;
 }
 
+// A thread's keys of a chunk of up to 32K tokens: every wave has 256 * rounds
+// consecutive ones (rounds: as few as cover the sequence), in the order (i, lane, c).
+constexpr uint32_t kLaneKeys = 8, kChunkKeys = kPickThreads * 4 * kLaneKeys;
+struct LaneKeys {
+  u32x4_e k[kLaneKeys];
+  uint32_t rounds, first;  // first: the wave's first token
+  __device__ __forceinline__ uint32_t token(uint32_t i, uint32_t c) const { return first + i * 256u + (threadIdx.x & 63u) * 4u + c; }
+  // All loads at once.  Past the last token the scratch holds anything.
+  __device__ __forceinline__ void load(const uint32_t* keys, uint32_t chunk, uint32_t tokens, uint32_t stride) {
+    rounds = tokens >= kChunkKeys ? kLaneKeys : (tokens + kPickThreads * 4u - 1u) / (kPickThreads * 4u);
+    first = chunk * kChunkKeys + uint32_t(__builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6))) * (256u * rounds);
+#pragma unroll
+    for (uint32_t i = 0; i < kLaneKeys; ++i) {
+      const uint32_t t = token(i, 0u);
+      k[i] = i < rounds && t < stride ? *reinterpret_cast<const u32x4_e*>(keys + t) : u32x4_e{0u, 0u, 0u, 0u};
+    }
+  }
+};
+
 __global__ __launch_bounds__(kPickThreads) void evict_pick_kernel(const EvictArgs a) {
-  __shared__ uint32_t hist[kBins];
+  __shared__ uint32_t hist[kCopies][kBins];
   __shared__ uint32_t found[2], wave_gt[kPickWaves], wave_eq[kPickWaves];
   const uint32_t b = blockIdx.x, tid = threadIdx.x, lane = tid & 63u;
   const uint32_t wave = uint32_t(__builtin_amdgcn_readfirstlane(int(tid >> 6)));
+  const ScoredSeq e = evict_seq(a, b);
+  const uint32_t n = e.tokens < a.keep ? e.tokens : a.keep;
+  uint32_t* kept = a.kept + uint64_t(b) * a.keep;
+  const uint32_t* keys = a.scratch + uint64_t(b) * a.scratch_stride;
+  const uint32_t chunks = (e.tokens + kChunkKeys - 1u) / kChunkKeys;
+  LaneKeys own;
+  if (n < e.tokens) own.load(keys, 0u, e.tokens, a.scratch_stride);
   if (wave == 0u) {  // tokens kept before this sequence; the last one also closes the list
     uint32_t sum = 0;
     for (uint32_t i = lane; i < b; i += 64u) {
@@ -58,20 +90,13 @@ __global__ __launch_bounds__(kPickThreads) void evict_pick_kernel(const EvictArg
     for (int o = 32; o > 0; o >>= 1) sum += uint32_t(__shfl_xor(int(sum), o));
     if (lane == 0u) {
       a.kept_starts[b] = sum;
-      if (b + 1u == a.batch) {
-        const uint32_t t = evict_seq(a, b).tokens;
-        a.kept_starts[a.batch] = sum + (t < a.keep ? t : a.keep);
-      }
+      if (b + 1u == a.batch) a.kept_starts[a.batch] = sum + n;
     }
   }
-  const ScoredSeq e = evict_seq(a, b);
-  const uint32_t n = e.tokens < a.keep ? e.tokens : a.keep;
-  uint32_t* kept = a.kept + uint64_t(b) * a.keep;
   if (n == e.tokens) {
     for (uint32_t t = tid; t < n; t += kPickThreads) kept[t] = t;
     return;
   }
-  const uint32_t* keys = a.scratch + uint64_t(b) * a.max_tokens;
 
   // The n-th largest key: its digits from the top, `want` its rank among the
   // keys that share the digits found so far.
@@ -79,35 +104,39 @@ __global__ __launch_bounds__(kPickThreads) void evict_pick_kernel(const EvictArg
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
     const uint32_t digits = pass == 2 ? 1024u : kBins;
-    for (uint32_t i = tid; i < kBins; i += kPickThreads) hist[i] = 0u;
+    for (uint32_t i = tid; i < kCopies * kBins; i += kPickThreads) (&hist[0][0])[i] = 0u;
     __syncthreads();
-    for (uint32_t t = tid; t < e.tokens; t += kPickThreads) {
-      const uint32_t key = keys[t];
-      if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & (digits - 1u)], 1u);
+    uint32_t* const h = hist[wave % kCopies];
+    for (uint32_t chunk = 0; chunk < chunks; ++chunk) {
+      if (chunks > 1u) own.load(keys, chunk, e.tokens, a.scratch_stride);
+#pragma unroll
+      for (uint32_t i = 0; i < kLaneKeys; ++i) {
+        if (i >= own.rounds) break;
+#pragma unroll
+        for (uint32_t c = 0; c < 4u; ++c)
+          if (own.token(i, c) < e.tokens && (own.k[i][c] & mask) == prefix)
+            atomicAdd(&h[(own.k[i][c] >> shift) & (digits - 1u)], 1u);
+      }
     }
     __syncthreads();
-    if (wave == 0u) {  // lane l: bins from the top, digits / 64 each
-      const uint32_t per = digits / 64u, top = digits - 1u - lane * per;
-      uint32_t sum = 0;
-      for (uint32_t i = 0; i < per; ++i) sum += hist[top - i];
-      uint32_t upto = sum;
+    // Thread t has the bins top - 2 t and the next below (one bin in the last
+    // pass): keys in them, in the wave's bins up to them, in the waves before.
+    const uint32_t per = digits / kPickThreads, bin = digits - 1u - tid * per;
+    uint32_t c0 = 0, c1 = 0;
 #pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t v = uint32_t(__shfl_up(int(upto), o));
-        if (lane >= uint32_t(o)) upto += v;
-      }
-      uint32_t before = upto - sum;
-      if (before < want && want <= upto) {
-        for (uint32_t i = 0; i < per; ++i) {
-          const uint32_t c = hist[top - i];
-          if (want <= before + c) {
-            found[0] = top - i;
-            found[1] = want - before;
-            break;
-          }
-          before += c;
-        }
-      }
+    for (uint32_t c = 0; c < kCopies; ++c) {
+      c0 += hist[c][bin];
+      c1 += per == 2u ? hist[c][bin - 1u] : 0u;
+    }
+    const uint32_t upto = wave_scan(c0 + c1);
+    if (lane == 63u) wave_gt[wave] = upto;
+    __syncthreads();
+    uint32_t before = upto - c0 - c1;
+    for (uint32_t w = 0; w < wave; ++w) before += wave_gt[w];
+    if (before < want && want <= before + c0 + c1) {
+      const bool second = want > before + c0;
+      found[0] = second ? bin - 1u : bin;
+      found[1] = want - before - (second ? c0 : 0u);
     }
     __syncthreads();
     prefix |= found[0] << shift;
@@ -116,43 +145,99 @@ __global__ __launch_bounds__(kPickThreads) void evict_pick_kernel(const EvictArg
     __syncthreads();
   }
 
-  // Every wave counts, then writes, its contiguous share in order.
-  const uint32_t steps = (e.tokens + 63u) / 64u, per = (steps + kPickWaves - 1u) / kPickWaves;
-  const uint32_t s0 = wave * per < steps ? wave * per : steps, s1 = s0 + per < steps ? s0 + per : steps;
-  uint32_t gt = 0, eq = 0;
-  for (uint32_t s = s0; s < s1; ++s) {
-    const uint32_t t = s * 64u + lane;
-    const uint32_t key = t < e.tokens ? keys[t] : 0u;
-    gt += uint32_t(__popcll(__ballot(t < e.tokens && key > prefix)));
-    eq += uint32_t(__popcll(__ballot(t < e.tokens && key == prefix)));
-  }
-  if (lane == 0u) {
-    wave_gt[wave] = gt;
-    wave_eq[wave] = eq;
-  }
-  __syncthreads();
-  uint32_t eq_before = 0, at = 0;
-  for (uint32_t w = 0; w < wave; ++w) {
-    const uint32_t room = want > eq_before ? want - eq_before : 0u;
-    at += wave_gt[w] + (wave_eq[w] < room ? wave_eq[w] : room);
-    eq_before += wave_eq[w];
-  }
-  const uint64_t below = (uint64_t(1) << lane) - 1u;
-  for (uint32_t s = s0; s < s1; ++s) {
-    const uint32_t t = s * 64u + lane;
-    const uint32_t key = t < e.tokens ? keys[t] : 0u;
-    const bool is_eq = t < e.tokens && key == prefix;
-    const uint64_t eqs = __ballot(is_eq);
-    const bool stays = (t < e.tokens && key > prefix) || (is_eq && eq_before + uint32_t(__popcll(eqs & below)) < want);
-    const uint64_t all = __ballot(stays);
-    if (stays) kept[at + uint32_t(__popcll(all & below))] = t;
-    at += uint32_t(__popcll(all));
-    eq_before += uint32_t(__popcll(eqs));
+  // Chunk by chunk every wave counts its keys above the n-th and equal to it,
+  // then writes those that stay behind what the waves before it keep.
+  uint32_t at0 = 0, eq0 = 0;  // kept, and equal keys met, before the chunk
+  for (uint32_t chunk = 0; chunk < chunks; ++chunk) {
+    if (chunks > 1u) own.load(keys, chunk, e.tokens, a.scratch_stride);
+    uint32_t gt = 0, eq = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kLaneKeys; ++i)
+#pragma unroll
+      for (uint32_t c = 0; c < 4u; ++c) {
+        const bool in = i < own.rounds && own.token(i, c) < e.tokens;
+        gt += in && own.k[i][c] > prefix ? 1u : 0u;
+        eq += in && own.k[i][c] == prefix ? 1u : 0u;
+      }
+    const uint32_t all_gt = uint32_t(__builtin_amdgcn_readlane(int(wave_scan(gt)), 63));
+    const uint32_t all_eq = uint32_t(__builtin_amdgcn_readlane(int(wave_scan(eq)), 63));
+    if (lane == 0u) {
+      wave_gt[wave] = all_gt;
+      wave_eq[wave] = all_eq;
+    }
+    __syncthreads();
+    uint32_t at = at0, eqs = eq0;
+    for (uint32_t w = 0; w < kPickWaves; ++w) {
+      const uint32_t room = want > eq0 ? want - eq0 : 0u, take = wave_gt[w] + (wave_eq[w] < room ? wave_eq[w] : room);
+      if (w < wave) {
+        at += take;
+        eqs += wave_eq[w];
+      }
+      at0 += take;
+      eq0 += wave_eq[w];
+    }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t i = 0; i < kLaneKeys; ++i) {
+      if (i >= own.rounds) break;
+      uint32_t lane_eq = 0;
+      bool is_eq[4], is_gt[4];
+#pragma unroll
+      for (uint32_t c = 0; c < 4u; ++c) {
+        const bool in = i < own.rounds && own.token(i, c) < e.tokens;
+        is_gt[c] = in && own.k[i][c] > prefix;
+        is_eq[c] = in && own.k[i][c] == prefix;
+        lane_eq += is_eq[c] ? 1u : 0u;
+      }
+      const uint32_t eq_upto = wave_scan(lane_eq);
+      uint32_t rank = eqs + eq_upto - lane_eq, lane_stays = 0;
+      bool stays[4];
+#pragma unroll
+      for (uint32_t c = 0; c < 4u; ++c) {
+        stays[c] = is_gt[c] || (is_eq[c] && rank < want);
+        rank += is_eq[c] ? 1u : 0u;
+        lane_stays += stays[c] ? 1u : 0u;
+      }
+      const uint32_t upto = wave_scan(lane_stays);
+      uint32_t to = at + upto - lane_stays;
+#pragma unroll
+      for (uint32_t c = 0; c < 4u; ++c)
+        if (stays[c]) kept[to++] = own.token(i, c);
+      at += uint32_t(__builtin_amdgcn_readlane(int(upto), 63));
+      eqs += uint32_t(__builtin_amdgcn_readlane(int(eq_upto), 63));
+    }
   }
 }
 
 // Rows of a destination token: where it comes from and goes to, ~0 if nowhere.
 constexpr uint32_t kMoveTokens = 64;
+
+// Pieces P of the rows of `row_bytes` at p, every thread's loads of all of them
+// before any store: with a loop of load and store for each array the move of
+// 65,536 tokens took 69 us.
+template <typename P, uint32_t ROW_BYTES>
+struct Pieces {
+  static constexpr uint32_t kPer = ROW_BYTES / uint32_t(sizeof(P)), kN = (kMoveTokens * kPer + 255u) / 256u;
+  P v[kN];
+  template <typename F>
+  __device__ __forceinline__ void load(const void* p, F row) {
+#pragma unroll
+    for (uint32_t k = 0; k < kN; ++k) {
+      const uint32_t i = threadIdx.x + 256u * k;
+      const uint64_t at = row(i / kPer);
+      if (at != ~0ull) v[k] = *reinterpret_cast<const P*>(static_cast<const uint8_t*>(p) + at * ROW_BYTES + i % kPer * sizeof(P));
+    }
+  }
+  template <typename F>
+  __device__ __forceinline__ void store(void* p, F row) const {
+#pragma unroll
+    for (uint32_t k = 0; k < kN; ++k) {
+      const uint32_t i = threadIdx.x + 256u * k;
+      const uint64_t at = row(i / kPer);
+      if (at != ~0ull) *reinterpret_cast<P*>(static_cast<uint8_t*>(p) + at * ROW_BYTES + i % kPer * sizeof(P)) = v[k];
+    }
+  }
+};
 
 template <int BITS, int G>
 __global__ __launch_bounds__(256) void evict_move_kernel(const EvictArgs a) {
@@ -188,64 +273,67 @@ __global__ __launch_bounds__(256) void evict_move_kernel(const EvictArgs a) {
     to_slot[tid] = ts;
   }
   __syncthreads();
+  // Row numbers; ~0 past the last token and where there is no destination.
   const auto row = [&](uint32_t page, uint32_t slot) { return (uint64_t(page) * a.kv_heads + kv) * a.page_tokens + slot; };
-  // Pieces of `bytes` of both K and V rows of `row_bytes`.
-  const auto copy = [&](const void* p, uint32_t row_bytes, auto piece) {
-    using P = decltype(piece);
-    const uint32_t per = row_bytes / uint32_t(sizeof(P));
-    uint8_t* base = static_cast<uint8_t*>(const_cast<void*>(p));
-    for (uint32_t i = tid; i < count * per; i += 256u) {
-      const uint32_t t = i / per, x = i % per;
-      if (to_page[t] == 0xffffffffu) continue;
-      const P v = *reinterpret_cast<const P*>(base + row(from_page[t], from_slot[t]) * row_bytes + x * sizeof(P));
-      *reinterpret_cast<P*>(base + row(to_page[t], to_slot[t]) * row_bytes + x * sizeof(P)) = v;
-    }
-  };
+  const auto from = [&](uint32_t t) { return t < kMoveTokens && to_page[t] != 0xffffffffu ? row(from_page[t], from_slot[t]) : ~0ull; };
+  const auto to = [&](uint32_t t) { return t < kMoveTokens && to_page[t] != 0xffffffffu ? row(to_page[t], to_slot[t]) : ~0ull; };
+  Pieces<float, 4> w;
+  if (a.weights) w.load(a.weights, from);
   if constexpr (BITS == 4) {
-    copy(a.k, D / 2u, u32x4_e{});
-    copy(a.v, D / 2u, u32x4_e{});
-    if constexpr (G == 2) {
-      copy(a.k_scales, 8u, uint64_t{});
-      copy(a.v_scales, 8u, uint64_t{});
-    } else {
-      copy(a.k_scales, 4u * G, u32x4_e{});
-      copy(a.v_scales, 4u * G, u32x4_e{});
-    }
+    Pieces<u32x4_e, D / 2u> k, v;
+    Pieces<uint64_t, 4u * G> ks, vs;
+    k.load(a.k, from);
+    v.load(a.v, from);
+    ks.load(a.k_scales, from);
+    vs.load(a.v_scales, from);
+    k.store(a.k, to);
+    v.store(a.v, to);
+    ks.store(a.k_scales, to);
+    vs.store(a.v_scales, to);
   } else {
-    copy(a.k, D, u32x4_e{});
-    copy(a.k_scales, 4u, uint32_t{});
-    copy(a.v_scales, 4u, uint32_t{});
-    // Four tokens of a dim to a dword: j0 and page_tokens are multiples of 8,
+    Pieces<u32x4_e, D> k;
+    Pieces<float, 4> ks, vs;
+    k.load(a.k, from);
+    ks.load(a.k_scales, from);
+    vs.load(a.v_scales, from);
+    // V: four tokens of a dim to a dword: j0 and page_tokens are multiples of 8,
     // so the four slots are one aligned dword of one page.  The last, partial
     // four go byte by byte: the slots behind are not this call's.
     uint8_t* v = static_cast<uint8_t*>(a.v);
     const auto place = [&](uint32_t page, uint32_t slot, uint32_t d) {
       return ((uint64_t(page) * a.kv_heads + kv) * D + d) * a.page_tokens + slot;
     };
-    const uint32_t quads = (count + 3u) / 4u;
-    for (uint32_t i = tid; i < 16u * D; i += 256u) {
-      const uint32_t qd = i % 16u, d = i / 16u;
-      if (qd >= quads || to_page[4u * qd] == 0xffffffffu) continue;
-      uint8_t x[4];
-      bool whole = 4u * qd + 4u <= count;
+    const uint32_t qd = tid % 16u, t0 = 4u * qd;
+    bool in[4], whole = true;
 #pragma unroll
-      for (uint32_t k = 0; k < 4u; ++k) {
-        const uint32_t t = 4u * qd + k;
-        const bool in = t < count && to_page[t] != 0xffffffffu;
-        whole = whole && in;
-        x[k] = in ? v[place(from_page[t], from_slot[t], d)] : uint8_t(0);
-      }
-      uint8_t* dst = v + place(to_page[4u * qd], to_slot[4u * qd], d);
-      if (whole) {
-        *reinterpret_cast<uint32_t*>(dst) = uint32_t(x[0]) | uint32_t(x[1]) << 8 | uint32_t(x[2]) << 16 | uint32_t(x[3]) << 24;
-      } else {
+    for (uint32_t c = 0; c < 4u; ++c) {
+      in[c] = to_page[t0 + c] != 0xffffffffu;
+      whole = whole && in[c];
+    }
+    constexpr uint32_t kDims = D / 16u < 8u ? D / 16u : 8u;  // of a thread at once
+    for (uint32_t d0 = tid / 16u; d0 < D; d0 += 16u * kDims) {
+      uint8_t x[kDims][4];
 #pragma unroll
-        for (uint32_t k = 0; k < 4u; ++k)
-          if (4u * qd + k < count && to_page[4u * qd + k] != 0xffffffffu) dst[k] = x[k];
+      for (uint32_t i = 0; i < kDims; ++i)
+#pragma unroll
+        for (uint32_t c = 0; c < 4u; ++c) x[i][c] = in[c] ? v[place(from_page[t0 + c], from_slot[t0 + c], d0 + 16u * i)] : uint8_t(0);
+#pragma unroll
+      for (uint32_t i = 0; i < kDims; ++i) {
+        if (whole) {
+          *reinterpret_cast<uint32_t*>(v + place(to_page[t0], to_slot[t0], d0 + 16u * i)) =
+              uint32_t(x[i][0]) | uint32_t(x[i][1]) << 8 | uint32_t(x[i][2]) << 16 | uint32_t(x[i][3]) << 24;
+        } else {
+#pragma unroll
+          for (uint32_t c = 0; c < 4u; ++c)
+            if (in[c]) v[place(to_page[t0 + c], to_slot[t0 + c], d0 + 16u * i)] = x[i][c];
+        }
       }
     }
+    k.store(a.k, to);
+    ks.store(a.k_scales, to);
+    vs.store(a.v_scales, to);
   }
-  if (a.weights) copy(a.weights, 4u, uint32_t{});
+  if (a.weights) w.store(a.weights, to);
 }
 
 }  // namespace

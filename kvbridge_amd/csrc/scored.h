@@ -68,6 +68,8 @@ __device__ __forceinline__ int bci(int x) {
   return __builtin_amdgcn_mov_dpp(x, 0x150 + J, 0xF, 0xF, true);
 }
 
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return uint32_t(__builtin_amdgcn_readfirstlane(int(x))); }
+
 template <int I, int N, typename F>
 __device__ __forceinline__ void unrolled(F&& f) {
   if constexpr (I < N) {

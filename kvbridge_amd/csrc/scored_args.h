@@ -33,7 +33,7 @@ struct ScoredArgs {
   uint32_t q_stride, q_type, out_type, window, kv_bits;
   float scale, cap;
   float* weights;
-  uint32_t fresh, chunk_tiles, chunks;  // weights: tiles per work-group, work-groups per sequence
+  uint32_t fresh;
 };
 
 hipError_t launch_scored_attend(const ScoredArgs& a, hipStream_t stream);
@@ -82,6 +82,7 @@ struct EvictArgs {
   int64_t* positions;
   uint32_t batch, kv_heads, dim, page_tokens, pages, max_tokens, total_tokens, table_entries, dst_entries;
   uint32_t keep, sink, recent, kv_bits;
+  uint32_t scratch_stride;  // keys of a sequence, a multiple of 4
 };
 hipError_t launch_evict_select(const EvictArgs& a, hipStream_t stream);
 hipError_t launch_evict_move(const EvictArgs& a, hipStream_t stream);

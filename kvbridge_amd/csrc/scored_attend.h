@@ -422,7 +422,6 @@ struct AttendPlan {
   int back[16];
   int64_t qref;
 };
-__device__ __forceinline__ uint32_t uniform(uint32_t x) { return uint32_t(__builtin_amdgcn_readfirstlane(int(x))); }
 
 // Waves per SIMD that the registers allow without spills.
 template <class C, bool ONE>

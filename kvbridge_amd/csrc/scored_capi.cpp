@@ -100,6 +100,8 @@ int sized(const kvb_scored_shape* s, T* out, F&& f) {
 
 const char* kNullShape = "shape pointer must be non-null";
 
+uint32_t key_stride(const kvb_evict_shape& s) { return (s.max_tokens + 3) / 4 * 4; }
+
 kvb::EvictArgs evict_args(const kvb_evict_shape& s, const kvb_evict_input& in) {
   kvb::EvictArgs a{};
   a.seq_starts = in.seq_starts;
@@ -119,6 +121,7 @@ kvb::EvictArgs evict_args(const kvb_evict_shape& s, const kvb_evict_input& in) {
   a.sink = s.sink;
   a.recent = s.recent;
   a.kv_bits = s.kv_bits;
+  a.scratch_stride = key_stride(s);
   return a;
 }
 
@@ -210,9 +213,11 @@ int kvb_accumulate_weights(const kvb_scored_shape* s, const kvb_scored_input* in
     if (!m || !l || !weights) return invalid("m, l and weights must be non-null device buffers");
     if (const char* e = scored_input_error(*s, *in, false)) return invalid(e);
     kvb::ScoredArgs a = scored_args(*s, *in);
-    const kvb::ScoredChunks c = kvb::scored_chunks(*s);
-    a.chunks = c.chunks;
-    a.chunk_tiles = c.tiles;
+    const kvb::ScoredSplits p = kvb::weight_splits(*s);
+    a.items = p.items;
+    a.splits = p.splits;
+    a.split_tiles = p.tiles;
+    a.waves = p.waves;
     a.m = const_cast<float*>(m);
     a.l = const_cast<float*>(l);
     a.weights = weights;
@@ -227,7 +232,7 @@ int kvb_evict_scratch_elements(const kvb_evict_shape* s, size_t* elements) {
   return guarded([&]() -> int {
     if (!s || !elements) return invalid("shape and output pointers must be non-null");
     if (const char* e = kvb::evict_error(*s)) return invalid(e);
-    *elements = size_t(s->batch) * s->max_tokens;
+    *elements = size_t(s->batch) * key_stride(*s);
     return KVB_OK;
   });
 }
@@ -239,6 +244,7 @@ int kvb_evict_select(const kvb_evict_shape* s, const kvb_evict_input* in, const 
     if (const char* e = kvb::evict_error(*s)) return invalid(e);
     if (!in->seq_starts || !in->page_offsets || !in->page_table || !weights || !scratch || !kept || !kept_starts)
       return invalid("eviction buffers must be non-null");
+    if (off16(scratch)) return invalid("eviction scratch must be 16-byte aligned");
     kvb::EvictArgs a = evict_args(*s, *in);
     a.weights_in = weights;
     a.scratch = scratch;

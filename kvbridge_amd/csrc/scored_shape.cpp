@@ -56,23 +56,21 @@ uint32_t resident_waves(const kvb_scored_shape& s) {
   return s.dim == 256 || half || (s.kv_bits == 8 && s.page_tokens % 32 != 0) ? 8 : 12;
 }
 
-}  // namespace
-
-// Work items.  Where the caller names no split size, there are as many as fit
+// Work items; others: kv heads times blocks.  Where the caller names no split size, there are as many as fit
 // the GPU at once and the kernel shares them out over the sequences by length
 // (scored.h, item_of): every work-group then has about the same number of tiles
 // and pays for its start and end once.  An item is a whole CU's unless the
 // sequences are so many that rounding to whole items would idle over a
 // sixteenth of them; then work-groups have four waves.
-ScoredSplits scored_splits(const kvb_scored_shape& s) {
+ScoredSplits split_items(const kvb_scored_shape& s, uint64_t others, uint32_t split_tokens) {
   const uint64_t seen = s.window == 0 ? s.max_tokens
                                       : std::min<uint64_t>(s.max_tokens, uint64_t(s.window) + s.rows + 32);
-  const uint64_t tiles = (seen + 31) / 32, others = uint64_t(s.kv_heads) * scored_blocks(s);
+  const uint64_t tiles = (seen + 31) / 32;
   const uint32_t all = resident_waves(s);
   const uint32_t waves = s.batch * 8 <= std::max<uint64_t>(8, kCus / others) ? all : 4;
   const uint64_t resident = kCus * (all / waves);
-  if (s.split_tokens != 0 || s.batch > 256) {
-    uint64_t per = s.split_tokens / 32;
+  if (split_tokens != 0 || s.batch > 256) {
+    uint64_t per = split_tokens / 32;
     if (per == 0) {
       const uint64_t splits = std::max<uint64_t>(1, resident * 2 / (others * s.batch));
       per = std::max<uint64_t>(16, (tiles + splits - 1) / splits);
@@ -84,6 +82,12 @@ ScoredSplits scored_splits(const kvb_scored_shape& s) {
   const uint64_t least = 16, useful = s.batch * ((tiles + least - 1) / least);
   const uint64_t items = std::max<uint64_t>(s.batch, std::min(useful, resident / others));
   return ScoredSplits{uint32_t(items), s.batch == 1 ? uint32_t(items) : 0, uint32_t(least), waves};
+}
+
+}  // namespace
+
+ScoredSplits scored_splits(const kvb_scored_shape& s) {
+  return split_items(s, uint64_t(s.kv_heads) * scored_blocks(s), s.split_tokens);
 }
 
 // One work-group's merge reads the partials of up to 16 head-rows past its L2,
@@ -129,13 +133,6 @@ const char* evict_error(const kvb_evict_shape& s) {
   return nullptr;
 }
 
-// Tiles per work-group of the weights: four per wave, more where the grid
-// would otherwise hold over 4096 work-groups.
-ScoredChunks scored_chunks(const kvb_scored_shape& s) {
-  const uint64_t tiles = (uint64_t(s.max_tokens) + 31) / 32, others = uint64_t(s.batch) * s.kv_heads;
-  const uint64_t most = std::max<uint64_t>(1, 4096 / others);
-  const uint64_t per = std::max<uint64_t>(16, (tiles + most - 1) / most);
-  return ScoredChunks{uint32_t((tiles + per - 1) / per), uint32_t(per)};
-}
+ScoredSplits weight_splits(const kvb_scored_shape& s) { return split_items(s, s.kv_heads, 0); }
 
 }  // namespace kvb

@@ -25,9 +25,7 @@ ScoredSplits scored_splits(const kvb_scored_shape& s);
 // Whether the last work-group of a block merges its splits itself.
 bool scored_one_launch(const kvb_scored_shape& s, const ScoredSplits& p);
 
-struct ScoredChunks {
-  uint32_t chunks, tiles;  // work-groups per sequence and kv head, tiles of each
-};
-ScoredChunks scored_chunks(const kvb_scored_shape& s);
+// The same for the weights, whose work-groups take all blocks of a kv head.
+ScoredSplits weight_splits(const kvb_scored_shape& s);
 
 }  // namespace kvb

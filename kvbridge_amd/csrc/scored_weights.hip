@@ -1,19 +1,22 @@
 // Attention weights per cached token (kvb_accumulate_weights).
 //
 // With m and l of an attention call known, the weight of token t for head-row
-// r is exp(s_rt - m_r) / l_r: K is read once more, V not at all.  A work-group
-// of four waves takes chunk_tiles tiles of one (sequence, kv head), its waves
-// every fourth tile, so that a (page, kv head, slot) of a sequence is written
-// by one wave only and in one order.  The operands of as many blocks of 16
-// head-rows as fit 64 KiB of LDS are staged at once and a tile's K serves all
-// of them; more head-rows take another pass over the chunk.  The sum over
-// the head-rows of a block is a DPP reduction over the 16 lanes of a row.
+// r is exp(s_rt - m_r) / l_r: K is read once more, V not at all.  The items are
+// those of the attention (scored.h, item_of) over the tiles that any row sees, a
+// work-group's waves take an item's tiles in turn, so that a (page, kv head,
+// slot) of a sequence is written by one wave only and in one order.  The
+// operands of as many blocks of 16 head-rows as fit 64 KiB of LDS are staged at
+// once and a tile's K serves all of them; more head-rows take another pass over
+// the item.  The sum over the head-rows of a block is a DPP reduction over the
+// 16 lanes of a row.
 #include "scored.h"
 
 namespace kvb {
 namespace {
 
-constexpr uint32_t kWeightWaves = 4;
+// Waves per SIMD that the registers allow.
+template <class C>
+constexpr int kWeightOccupancy = C::kGroups == 8 || (C::kF > 1 && C::kH > 1) ? 2 : 3;
 
 __device__ __forceinline__ float row_sum16(float x) {
   x += row_ror<8>(x);
@@ -30,30 +33,67 @@ struct WeightBlock {
   uint32_t lo[16], hi[16];
   float m[16], per_l[16], slope[16];
   int back[16];
-  uint32_t min_lo, max_hi;
 };
 template <class C, int QD>
 constexpr uint32_t kBlocksAtOnce = 65536u / sizeof(WeightBlock<C, QD>);
 
 template <class C, int QD, bool ONE>
-__global__ __launch_bounds__(64 * kWeightWaves) void scored_weights_kernel(const ScoredArgs a) {
+__global__ __launch_bounds__((256 * kWeightOccupancy<C>), (kWeightOccupancy<C>)) void scored_weights_kernel(const ScoredArgs a) {
   extern __shared__ __align__(16) uint8_t lds_raw[];
   using Block = WeightBlock<C, QD>;
   Block* const blocks = reinterpret_cast<Block*>(lds_raw);
-  const uint32_t lane = threadIdx.x & 63u, r = lane & 15u, kg = lane >> 4;
-  const uint32_t wave = uint32_t(__builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6)));
-  uint32_t at = blockIdx.x;
-  const uint32_t kv = at % a.kv_heads;
-  at /= a.kv_heads;
-  const uint32_t chunk = at % a.chunks, b = at / a.chunks;
-  const ScoredSeq e = clamp_seq(a.seq_starts[b], a.seq_starts[b + 1u], a.page_offsets[b], a.total_tokens, a.table_entries,
-                                a.page_tokens, a.max_tokens);
-  const uint32_t tiles = e.tokens / kTileTokens + (e.tokens % kTileTokens != 0u ? 1u : 0u);
-  const uint64_t c0 = uint64_t(chunk) * a.chunk_tiles;
-  if (c0 >= tiles) return;
-  const uint32_t t_begin = uint32_t(c0), t_end = tiles - t_begin > a.chunk_tiles ? t_begin + a.chunk_tiles : tiles;
+  __shared__ WorkItem plan_it;
+  __shared__ uint32_t plan_found, plan_pre, plan_lo, plan_hi;
+  const uint32_t lane = threadIdx.x & 63u, r = lane & 15u, kg = lane >> 4, NW = blockDim.x >> 6;
+  const uint32_t wave = uniform(threadIdx.x >> 6);
+  const uint32_t kv = blockIdx.x % a.kv_heads, item = blockIdx.x / a.kv_heads;
+  if (wave == 0u) {
+    WorkItem w{0u, 0u, 0u, 0u, ScoredSeq{0u, 0u, 0u}};
+    const bool found = item_of(a, item, w);
+    if (lane == 0u) {
+      plan_it = w;
+      plan_found = found && w.e.tokens > 0u ? 1u : 0u;
+    }
+  }
+  const uint32_t at_once = a.blocks < kBlocksAtOnce<C, QD> ? a.blocks : kBlocksAtOnce<C, QD>;
+  for (uint32_t i = 0; i < at_once; ++i) clear_q(blocks[i].q, threadIdx.x, 64u * NW);
+  __syncthreads();
+  if (uniform(plan_found) == 0u) return;
+  const uint32_t b = uniform(plan_it.seq), split = uniform(plan_it.split), shares = uniform(plan_it.count);
+  const ScoredSeq e{uniform(plan_it.e.start), uniform(plan_it.e.tokens), uniform(plan_it.e.table_off)};
+  const uint32_t tiles = (e.tokens - 1u) / kTileTokens + 1u;
   const uint32_t fresh0 = a.fresh < e.tokens ? e.tokens - a.fresh : 0u;  // tokens from here on are set
-  const int64_t qref = a.q_positions[uint64_t(b) * a.rows], prefix = a.prefix ? a.prefix[b] : 0;
+  const int64_t* q_positions = a.q_positions + uint64_t(b) * a.rows;
+  const int64_t qref = q_positions[0], prefix = a.prefix ? a.prefix[b] : 0;
+  const auto share = [&](uint32_t n) {
+    const uint32_t per = n / shares + (n % shares != 0u ? 1u : 0u);
+    return per > a.split_tiles ? per : a.split_tiles;
+  };
+
+  // The tokens that any row sees, by the last wave: one row per lane.
+  if (wave == NW - 1u) {
+    uint32_t lo = 0xffffffffu, hi = 0u, pre = 0u;
+    for (uint32_t row0 = 0; row0 < a.rows; row0 += 64u) {
+      const bool valid = row0 + lane < a.rows;
+      const Visible v = visible_tokens(a, e, valid, ask_visible(a, e, q_positions[valid ? row0 + lane : 0u], prefix));
+      if (v.lo < v.hi) {
+        lo = v.lo < lo ? v.lo : lo;
+        hi = v.hi > hi ? v.hi : hi;
+      }
+      pre = v.pre;
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+      const uint32_t l2 = uint32_t(__shfl_xor(int(lo), o)), h2 = uint32_t(__shfl_xor(int(hi), o));
+      lo = l2 < lo ? l2 : lo;
+      hi = h2 > hi ? h2 : hi;
+    }
+    if (lane == 0u) {
+      plan_pre = pre;
+      plan_lo = hi == 0u ? 0u : lo;
+      plan_hi = hi;
+    }
+  }
 
   for (uint32_t first = 0; first < a.blocks; first += kBlocksAtOnce<C, QD>) {
     const uint32_t count = a.blocks - first < kBlocksAtOnce<C, QD> ? a.blocks - first : kBlocksAtOnce<C, QD>;
@@ -61,91 +101,60 @@ __global__ __launch_bounds__(64 * kWeightWaves) void scored_weights_kernel(const
       __threadfence();  // what the first pass set is in place before it is added to
       __syncthreads();  // and every wave is done with the last pass's operands
     }
-    for (uint32_t i = 0; i < count; ++i) clear_q(blocks[i].q, threadIdx.x, 64u * kWeightWaves);
-    if (C::kF > 1) __syncthreads();
-    for (uint32_t i = 0; i < count; ++i) {
-      const uint32_t hr = (first + i) * 16u + threadIdx.x / 16u;
+    // Q by groups of four waves, what else a head-row needs by single waves.
+    for (uint32_t i = wave >> 2; i < count; i += NW >> 2) {
+      const uint32_t tid = threadIdx.x & 255u, hr = (first + i) * 16u + tid / 16u;
       stage_q<C, QD>(a, (uint64_t(b) * a.rows + hr / a.group) * a.q_stride + uint64_t(kv * a.group + hr % a.group) * a.dim,
-                     hr < a.head_rows, blocks[i].q, threadIdx.x);
+                     hr < a.head_rows, blocks[i].q, tid);
     }
-    uint32_t pre = 0;
-    for (uint32_t i = wave; i < count; i += kWeightWaves) {
+    for (uint32_t i = wave; i < count; i += NW) {
       const uint32_t hr = (first + i) * 16u + r / C::kF;
       const bool valid = hr < a.head_rows;
       const uint32_t hrc = valid ? hr : a.head_rows - 1u;
       const uint32_t row = hrc / a.group, head = kv * a.group + hrc % a.group;
       const uint64_t rh = (uint64_t(b) * a.rows + row) * a.q_heads + head;
-      const int64_t qpos = a.q_positions[uint64_t(b) * a.rows + row];
+      const int64_t qpos = q_positions[row];
+      const float l = a.l[rh], m = a.m[rh];
       const Visible vis = visible_tokens(a, e, valid, ask_visible(a, e, qpos, prefix));
-      pre = vis.pre;
-      const float l = a.l[rh];
       const bool counts = valid && l > 0.f;
       Block& w = blocks[i];
       if (kg == 0u) {
         w.lo[r] = vis.lo;
         w.hi[r] = vis.hi;
-        w.m[r] = counts ? a.m[rh] : FLT_MAX;
+        w.m[r] = counts ? m : FLT_MAX;
         w.per_l[r] = counts && r % C::kF == 0u ? 1.f / l : 0.f;  // a head-row's F columns hold the same score
         w.slope[r] = a.slopes ? a.slopes[head] : 0.f;
         w.back[r] = near(int64_t(uint64_t(qpos) - uint64_t(qref)));
       }
-      if (lane == 0u) {
-        w.min_lo = vis.min_lo;
-        w.max_hi = vis.max_hi;
-      }
     }
-    if (wave >= count && a.prefix) pre = visible_tokens(a, e, false, ask_visible(a, e, 0, prefix)).pre;  // the same for every row
     __syncthreads();
-    uint32_t min_lo = 0xffffffffu, max_hi = 0u;
-    for (uint32_t i = 0; i < count; ++i) {
-      const uint32_t lo = blocks[i].min_lo, hi = blocks[i].max_hi;
-      if (hi > 0u && lo < min_lo) min_lo = lo;
-      if (hi > max_hi) max_hi = hi;
-    }
-    min_lo = uint32_t(__builtin_amdgcn_readfirstlane(int(min_lo)));
-    max_hi = uint32_t(__builtin_amdgcn_readfirstlane(int(max_hi)));
-
-    const auto live = [&](uint32_t t) {
-      const uint32_t t0 = t * kTileTokens;
-      return t0 < pre || (t0 < max_hi && t0 + kTileTokens > min_lo);
-    };
-    const auto next = [&](uint32_t t) {
-      while (t < t_end && !live(t) && !(first == 0u && t * kTileTokens + kTileTokens > fresh0)) t += kWeightWaves;
-      return t;
-    };
-    uint32_t t = next(t_begin + wave);
-    if (t >= t_end) continue;
-    // Page lookups of 16 of the wave's tiles at a time; tile t is its (t - t_begin) / 4-th.
+    const uint32_t pre = uniform(plan_pre);
+    const LiveTiles live = live_tiles(pre, uniform(plan_lo), uniform(plan_hi));
+    const uint32_t per = share(live.n);
+    const uint32_t t_first = split * per + wave;
+    const uint32_t t_end = split * per >= live.n ? 0u : (live.n - split * per > per ? split * per + per : live.n);
+    const uint32_t n = t_first < t_end ? (t_end - t_first + NW - 1u) / NW : 0u;
     const auto tile_of = [&](uint32_t i) {
-      const uint64_t x = uint64_t(t_begin) + wave + uint64_t(i) * kWeightWaves;
-      return x < tiles ? uint32_t(x) : tiles - 1u;
+      const uint64_t x = uint64_t(t_first) + uint64_t(i) * NW;
+      return live.tile(x < live.n ? uint32_t(x) : live.n - 1u);
     };
-    const auto number = [&](uint32_t tile) { return (tile - t_begin) / kWeightWaves; };
-    uint32_t window = number(t) / 16u;
-    TilePages pages = tile_pages(a, e, tile_of, window * 16u, lane), pages_next = tile_pages(a, e, tile_of, window * 16u + 16u, lane);
-    const auto rows_at = [&](uint32_t tile) {
-      const uint32_t w = number(tile) / 16u;
-      if (w != window) {
-        pages = w == window + 1u ? pages_next : tile_pages(a, e, tile_of, w * 16u, lane);
-        window = w;
-        pages_next = tile_pages(a, e, tile_of, w * 16u + 16u, lane);
-      }
-      return tile_rows<ONE>(a, pages, number(tile), kv);
-    };
-    TileRows<ONE> rows = rows_at(t);
-    int ahead = load_ahead<C>(a, e, t * kTileTokens, r, kg, qref);
-    typename C::K k = C::template load_k<ONE>(a, rows, r, kg, e.tokens - t * kTileTokens);
-    while (t < t_end) {
-      const uint32_t t1 = next(t + kWeightWaves), tl = t1 < t_end ? t1 : t;
-      const TileRows<ONE> rows1 = rows_at(tl);
-      const int ahead1 = load_ahead<C>(a, e, tl * kTileTokens, r, kg, qref);
-      const typename C::K k1 = C::template load_k<ONE>(a, rows1, r, kg, e.tokens - tl * kTileTokens);
-      const uint32_t t0 = t * kTileTokens;
-      float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (live(t)) {
-        for (uint32_t i = 0; i < count; ++i) {
+    if (n > 0u) {
+      TilePages pages = tile_pages(a, e, tile_of, 0u, lane), ahead_pages = pages;
+      TileRows<ONE> rows = tile_rows<ONE>(a, pages, 0u, kv);
+      uint32_t t0 = tile_of(0u) * kTileTokens;
+      typename C::K k = C::template load_k<ONE>(a, rows, r, kg, e.tokens - t0);
+      int ahead = load_ahead<C>(a, e, t0, r, kg, qref);
+      for (uint32_t i = 0; i < n; ++i) {
+        if (i % 16u == 0u) ahead_pages = tile_pages(a, e, tile_of, i + 16u, lane);
+        const uint32_t t_next = tile_of(i + 1u < n ? i + 1u : i) * kTileTokens;
+        if ((i + 1u) % 16u == 0u) pages = ahead_pages;
+        const TileRows<ONE> rows_next = tile_rows<ONE>(a, pages, i + 1u < n ? i + 1u : i, kv);
+        const typename C::K k_next = C::template load_k<ONE>(a, rows_next, r, kg, e.tokens - t_next);
+        const int ahead_next = load_ahead<C>(a, e, t_next, r, kg, qref);
+        float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        for (uint32_t bl = 0; bl < count; ++bl) {
           asm volatile("" ::: "memory");  // the operands stay in LDS: not hoisted out of the loops
-          const Block& w = blocks[i];
+          const Block& w = blocks[bl];
           float x[8];
           tile_scores<C, QD>(k, w.q, lane, x);
           const ScoreForm form = score_form(a, w.q.factor[r], w.slope[r], w.back[r]);
@@ -154,34 +163,47 @@ __global__ __launch_bounds__(64 * kWeightWaves) void scored_weights_kernel(const
 #pragma unroll
           for (int j = 0; j < 8; ++j) sum[j] = fmaf(per_l > 0.f ? exp_e(x[j] - m) : 0.f, per_l, sum[j]);
         }
+        float total = row_sum16(sum[0]);
+        unrolled<1, 8>([&](auto jc) {
+          const float s = row_sum16(sum[jc]);
+          total = r == uint32_t(jc) ? s : total;
+        });
+        const uint32_t in = C::token(kg, r % 8u), tok = t0 + in;
+        if (r < 8u && tok < e.tokens) {
+          const uint32_t P = a.page_tokens;
+          const uint64_t at = ONE ? rows.row(0, P) + in
+                                  : pick(in / 8u, rows.row(0, P), rows.row(ONE ? 0 : 1, P), rows.row(ONE ? 0 : 2, P), rows.row(ONE ? 0 : 3, P)) + in % 8u;
+          if (first == 0u && tok >= fresh0) a.weights[at] = total;
+          else unsafeAtomicAdd(a.weights + at, total);
+        }
+        k = k_next;
+        rows = rows_next;
+        t0 = t_next;
+        ahead = ahead_next;
       }
-      float total = row_sum16(sum[0]);
-      unrolled<1, 8>([&](auto jc) {
-        const float s = row_sum16(sum[jc]);
-        total = r == uint32_t(jc) ? s : total;
-      });
-      const uint32_t in = C::token(kg, r % 8u), tok = t0 + in;
-      if (r < 8u && tok < e.tokens) {
-        const uint32_t P = a.page_tokens;
-        const uint64_t row = ONE ? rows.row(0, P) + in
-                                 : pick(in / 8u, rows.row(0, P), rows.row(1, P), rows.row(2, P), rows.row(3, P)) + in % 8u;
-        if (first == 0u && tok >= fresh0) a.weights[row] = total;
-        else unsafeAtomicAdd(a.weights + row, total);
+    }
+    // Fresh tokens of the tiles that no row sees: 0.
+    if (first == 0u) {
+      const uint32_t live_end = live.first + (live.n - live.pre_tiles);
+      for (uint64_t t = uint64_t(fresh0 / kTileTokens) + split * NW + wave; t < tiles; t += uint64_t(shares) * NW) {
+        if (t < live.pre_tiles || (t >= live.first && t < live_end)) continue;
+        const uint32_t tok = uint32_t(t) * kTileTokens + lane;
+        if (lane >= kTileTokens || tok < fresh0 || tok >= e.tokens) continue;
+        const uint32_t lp = tok / a.page_tokens;
+        uint32_t page = a.page_table[e.table_off + lp];
+        page = page < a.pages ? page : a.pages - 1u;
+        a.weights[(uint64_t(page) * a.kv_heads + kv) * a.page_tokens + (tok - lp * a.page_tokens)] = 0.f;
       }
-      t = t1;
-      rows = rows1;
-      ahead = ahead1;
-      k = k1;
     }
   }
 }
 
 template <class C, int QD>
 hipError_t launch_digits(const ScoredArgs& a, hipStream_t stream) {
-  const uint32_t groups = a.batch * a.chunks * a.kv_heads;
+  const uint32_t groups = a.items * a.kv_heads, most = 4u * uint32_t(kWeightOccupancy<C>), waves = a.waves < most ? a.waves : most;
   const uint32_t bytes = uint32_t(sizeof(WeightBlock<C, QD>)) * (a.blocks < kBlocksAtOnce<C, QD> ? a.blocks : kBlocksAtOnce<C, QD>);
-  if (a.page_tokens % kTileTokens == 0u) scored_weights_kernel<C, QD, true><<<groups, 64 * kWeightWaves, bytes, stream>>>(a);
-  else scored_weights_kernel<C, QD, false><<<groups, 64 * kWeightWaves, bytes, stream>>>(a);
+  if (a.page_tokens % kTileTokens == 0u) scored_weights_kernel<C, QD, true><<<groups, 64u * waves, bytes, stream>>>(a);
+  else scored_weights_kernel<C, QD, false><<<groups, 64u * waves, bytes, stream>>>(a);
   return hipGetLastError();
 }
 template <class C>

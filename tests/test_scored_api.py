@@ -171,6 +171,8 @@ def test_evict_calls_rejected_before_launch():
         kvb.evict_select(s, inp, None, FAKE, FAKE, FAKE, stream=0)
     with pytest.raises(kvb.KvbInvalidArgument, match="eviction buffers"):
         kvb.evict_select(s, kvb.evict_input(FAKE, None, FAKE, None), FAKE, FAKE, FAKE, FAKE, stream=0)
+    with pytest.raises(kvb.KvbInvalidArgument, match="16-byte aligned"):
+        kvb.evict_select(s, inp, FAKE, FAKE + 4, FAKE, FAKE, stream=0)
     cache = [FAKE] * 8
     for i, x, msg in [(5, None, "eviction buffers"), (6, None, "eviction buffers"), (1, None, "cache buffers"),
                       (0, FAKE + 2, "16-byte aligned"), (3, FAKE + 4, "cache scales")]:
