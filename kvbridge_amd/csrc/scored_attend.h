@@ -63,60 +63,68 @@ __device__ __forceinline__ void store_out4(const ScoredArgs& a, uint64_t at, f32
 }
 
 // Running state of a wave: acc[f] columns are head-rows (times F), rows dims.
-// The reference is kept in units of log 2, where it is exact by definition: p =
-// exp2(fma(score, log2 e, -mref2)) rounds once.
+// The reference `ref` is a whole number of factors of 2, and so is ve, so that
+// both go into one exponent: w' = exp2(fma(score, log2 e, ve - ref)) rounds
+// once, and l, mid and the products all carry 2^(ve - ref).
 template <class C>
 struct AttendState {
   f32x4 acc[2 * C::kGroups];
   float mid[C::kBits == 4 ? C::kH : 1];
-  float mref2, mtop, l, vf;  // reference, maximum of the lane's scores, sum, 2^ve
+  float mtop, l;         // maximum of the lane's scores, sum
+  float ref, down, vf;   // reference, ve - reference, 2^ve
   int ve;
 };
-__device__ __forceinline__ float weight(float score, float mref2) {
-  return __builtin_amdgcn_exp2f(fmaf(score, kLog2e, -mref2));
+constexpr float kNoRef = -0x1p100f;  // below any score's exponent
+__device__ __forceinline__ float weight(float score, float down) {
+  return __builtin_amdgcn_exp2f(fmaf(score, kLog2e, down));
 }
-// exp(top) / 2^mref2 inverted: the factor from the reference to `top`, with the
-// rounding of top * log2 e taken back.
-__device__ __forceinline__ float to_top(float mref2, float top) {
-  const float t2 = top * kLog2e;
-  return __builtin_amdgcn_exp2f((mref2 - t2) - fmaf(top, kLog2e, -t2));
+// The factor from 2^(ve - ref) to exp(-top), the rounding of top * log2 e taken
+// back: 2^(ref - ve) / e^top as a fraction's exponential and a whole power.
+struct ToTop {
+  float fraction;
+  int power;
+};
+__device__ __forceinline__ ToTop to_top(float ref, int ve, float top) {
+  const float t2 = top * kLog2e, up = __builtin_ceilf(t2);
+  return ToTop{__builtin_amdgcn_exp2f((up - t2) - fmaf(top, kLog2e, -t2)), int(fmaxf(ref - up, -1000.f)) - ve};
 }
 
 // Moves the reference to the head-row's maximum and sets ve by the tile's
 // largest weight of the column.  mult(j): the largest step of the lane's token j.
 template <class C, typename F>
 __device__ __forceinline__ void rescale(AttendState<C>& s, const float (&x)[8], F mult) {
-  const float mref2 = fmaxf(s.mref2, rows_max(s.mtop) * kLog2e);
-  const float jump = mref2 - s.mref2;
-  const float alpha = __builtin_amdgcn_exp2f(-jump);
+  const float ref = fmaxf(s.ref, __builtin_ceilf(rows_max(s.mtop) * kLog2e));
+  const float jump = ref - s.ref;
   float w = 0.f;
   unrolled<0, 8>([&](auto jc) {
     constexpr int j = jc;
-    const float p = weight(x[j], mref2), big = mult(jc);
+    const float p = weight(x[j], -ref), big = mult(jc);
     w = fmaxf(w, p > 0.f ? p * big : 0.f);
   });
   w = rows_max(w);
   int ve = s.ve;
+  const int moved = int(fminf(jump, 2000.f));
   if (w > 0.f && w <= FLT_MAX) {
     // Upwards only as far as the reference moved: the numerators must not grow.
-    const int room = s.ve + int(fminf(jump, 200.f));
+    const int room = s.ve + (moved < 200 ? moved : 200);
     ve = -__builtin_amdgcn_frexp_expf(w);
     ve = ve < room ? ve : room;
-    ve = ve < -120 ? -120 : (ve > 120 ? 120 : ve);
+    ve = ve < -64 ? -64 : (ve > 64 ? 64 : ve);  // l and mid carry 2^ve
   }
-  const int dv = ve - s.ve;
+  const int dv = ve - s.ve - moved;  // 0 or less, or a score is not finite
 #pragma unroll
   for (int f = 0; f < 2 * C::kGroups; ++f)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) s.acc[f][i] = ldexpf(s.acc[f][i] * alpha, dv);
-  s.l *= alpha;
+    for (int i = 0; i < 4; ++i) s.acc[f][i] = ldexpf(s.acc[f][i], dv);
+  s.l = ldexpf(s.l, dv);
   if constexpr (C::kBits == 4) {
 #pragma unroll
-    for (int h = 0; h < C::kH; ++h) s.mid[h] *= alpha;
+    for (int h = 0; h < C::kH; ++h) s.mid[h] = ldexpf(s.mid[h], dv);
   }
-  s.mref2 = mref2;
+  s.ref = ref;
   s.ve = ve;
   s.vf = ldexpf(1.f, ve);
+  s.down = float(ve) - ref;
 }
 
 template <int PD>
@@ -140,14 +148,15 @@ __device__ __forceinline__ PDigits<PD> p_digits(const float (&w)[8]) {
 template <int G, int F>
 __device__ __forceinline__ void keep_range(const typename Cache4<G, F>::V& v, const float (&x)[8], AttendState<Cache4<G, F>>& s) {
   using C = Cache4<G, F>;
-  typename C::Params p;
-  float top = 0.f;
+  // The largest step as the largest word (of an integer: the low half may only
+  // add 2^-7; a NaN asks for the rescale too).
+  int most = int(v.p.w[0]);
 #pragma unroll
-  for (int i = 0; i < C::kPWords; ++i) {
-    p.step[i] = __uint_as_float(v.p.w[i] & 0xffff0000u);
-    top = fmaxf(top, p.step[i]);
-  }
-  if (!__any(fmaf(s.mtop, kLog2e, -s.mref2) > 8.f || top * s.vf > 128.f)) return;
+  for (int i = 1; i < C::kPWords; ++i) most = int(v.p.w[i]) > most ? int(v.p.w[i]) : most;
+  if (!__any(fmaf(s.mtop, kLog2e, -s.ref) > 8.f || !(__int_as_float(most) * s.vf <= 128.f))) return;
+  typename C::Params p;
+#pragma unroll
+  for (int i = 0; i < C::kPWords; ++i) p.step[i] = __uint_as_float(v.p.w[i] & 0xffff0000u);
   rescale(s, x, [&](auto jc) {
     constexpr int j = jc;
     float t = 0.f;
@@ -160,7 +169,7 @@ __device__ __forceinline__ void keep_range(const typename Cache4<G, F>::V& v, co
 }
 template <int G>
 __device__ __forceinline__ void keep_range(const typename Cache8<G>::V& v, const float (&x)[8], AttendState<Cache8<G>>& s) {
-  if (!__any(fmaf(s.mtop, kLog2e, -s.mref2) > 8.f || v.p * s.vf > 128.f)) return;
+  if (!__any(fmaf(s.mtop, kLog2e, -s.ref) > 8.f || !(v.p * s.vf <= 128.f))) return;
   rescale(s, x, [&](auto jc) {
     constexpr int j = jc;
     return bc<j>(v.p);
@@ -186,7 +195,7 @@ __device__ __forceinline__ void hide_odd_params(typename Cache4<G, F>::V& v, con
   if constexpr (F == 1) {
     uint32_t seen = 0u;  // bit 2 j: the lane's token j has a weight
 #pragma unroll
-    for (int j = 0; j < 8; ++j) seen |= weight(x[j], s.mref2) != 0.f ? 1u << (2 * j) : 0u;
+    for (int j = 0; j < 8; ++j) seen |= weight(x[j], s.down) != 0.f ? 1u << (2 * j) : 0u;
 #pragma unroll
     for (int i = 0; i < PW; ++i) {
       const uint32_t lanes = uint32_t(__ballot(odd[i]) >> (16u * kg));  // bit 2 j + h: token j, block h * PW + i
@@ -196,7 +205,7 @@ __device__ __forceinline__ void hide_odd_params(typename Cache4<G, F>::V& v, con
   } else {
 #pragma unroll
     for (int i = 0; i < PW; ++i)
-      s.mid[i % C::kH] = odd[i] && weight(x[i / C::kH], s.mref2) != 0.f ? nan : s.mid[i % C::kH];
+      s.mid[i % C::kH] = odd[i] && weight(x[i / C::kH], s.down) != 0.f ? nan : s.mid[i % C::kH];
   }
 #pragma unroll
   for (int i = 0; i < PW; ++i) v.p.w[i] = odd[i] ? 0u : v.p.w[i];
@@ -211,12 +220,9 @@ __device__ __forceinline__ void tile_values(const typename Cache4<G, F>::V& v, c
                                             AttendState<Cache4<G, F>>& s, uint32_t code_bits) {
   using C = Cache4<G, F>;
   const typename C::Params par = C::template unpack<true>(v.p);
-  float p[8], pv[8];
+  float p[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    p[j] = weight(x[j], s.mref2);
-    pv[j] = p[j] * s.vf;
-  }
+  for (int j = 0; j < 8; ++j) p[j] = weight(x[j], s.down);
   s.l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
   unrolled<0, C::kH>([&](auto hc) {
     constexpr int h = hc;
@@ -224,7 +230,7 @@ __device__ __forceinline__ void tile_values(const typename Cache4<G, F>::V& v, c
     unrolled<0, 8>([&](auto jc) {
       constexpr int j = jc;
       const float step = par.template step_of<j, h>(), at8 = par.template other_of<j, h>();
-      w[j] = step * pv[j];
+      w[j] = step * p[j];
       s.mid[h] = fmaf(at8, p[j], s.mid[h]);
     });
     const PDigits<PD> d = p_digits<PD>(w);
@@ -257,8 +263,8 @@ __device__ __forceinline__ void tile_values(const typename Cache8<G>::V& v, cons
   float p[8], w[8];
   unrolled<0, 8>([&](auto jc) {
     constexpr int j = jc;
-    p[j] = weight(x[j], s.mref2);
-    w[j] = bc<j>(v.p) * (p[j] * s.vf);
+    p[j] = weight(x[j], s.down);
+    w[j] = bc<j>(v.p) * p[j];
     w[j] = p[j] == 0.f ? 0.f : w[j];
   });
   s.l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
@@ -271,8 +277,8 @@ __device__ __forceinline__ void tile_values(const typename Cache8<G>::V& v, cons
   }
 }
 
-// Four consecutive dims of a lane's head-row in units of 2^mref2: chunk c of its
-// 2 H, and the first of its dims.
+// Four consecutive dims of a lane's head-row in units of 2^(ve - ref): chunk c
+// of its 2 H, and the first of its dims.
 template <int G, int F>
 __device__ __forceinline__ f32x4 chunk_value(const AttendState<Cache4<G, F>>& s, int c, const float (&mid)[G / F], uint32_t r) {
   constexpr int H = G / F;
@@ -285,14 +291,12 @@ __device__ __forceinline__ f32x4 chunk_value(const AttendState<Cache4<G, F>>& s,
       a[i] = r % F == uint32_t(f) ? s.acc[2 * (f * H + h)][i] : a[i];
       o[i] = r % F == uint32_t(f) ? s.acc[2 * (f * H + h) + 1][i] : o[i];
     }
-  const float even = ldexpf(1.f, -s.ve), odd = ldexpf(1.f, -4 - s.ve);
-  return f32x4{fmaf(a[2 * half], even, mid[h]), fmaf(o[2 * half], odd, mid[h]), fmaf(a[2 * half + 1], even, mid[h]),
-               fmaf(o[2 * half + 1], odd, mid[h])};
+  return f32x4{a[2 * half] + mid[h], fmaf(o[2 * half], 0.0625f, mid[h]), a[2 * half + 1] + mid[h],
+               fmaf(o[2 * half + 1], 0.0625f, mid[h])};
 }
 template <int G>
 __device__ __forceinline__ f32x4 chunk_value(const AttendState<Cache8<G>>& s, int c, const float (&)[1], uint32_t) {
-  const float f = ldexpf(1.f, -s.ve);
-  return f32x4{s.acc[c][0] * f, s.acc[c][1] * f, s.acc[c][2] * f, s.acc[c][3] * f};
+  return s.acc[c];
 }
 template <class C>
 __device__ __forceinline__ uint32_t chunk_dim(uint32_t c, uint32_t r, uint32_t kg) {
@@ -532,9 +536,10 @@ __global__ __launch_bounds__((256 * kAttendOccupancy<C, ONE>), (kAttendOccupancy
   for (int f = 0; f < 2 * C::kGroups; ++f) s.acc[f] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int h = 0; h < (C::kBits == 4 ? C::kH : 1); ++h) s.mid[h] = 0.f;
-  s.mref2 = -FLT_MAX;
   s.mtop = neg_inf();
   s.l = 0.f;
+  s.ref = kNoRef;
+  s.down = -kNoRef;
   s.vf = 1.f;
   s.ve = 0;
 
@@ -584,8 +589,9 @@ __global__ __launch_bounds__((256 * kAttendOccupancy<C, ONE>), (kAttendOccupancy
   __syncthreads();  // also: every wave is done with Q
   float top = lds_m[0][r];
   for (uint32_t w = 1; w < NW; ++w) top = fmaxf(top, lds_m[w][r]);
-  const float f = l == 0.f ? 0.f : to_top(s.mref2, top);  // a wave without visible tokens: 0
-  if (kg == 0u) lds_l[wave][r] = l * f;
+  const ToTop f = to_top(s.ref, s.ve, top);
+  // l = 0: a wave without visible tokens
+  if (kg == 0u) lds_l[wave][r] = l == 0.f ? 0.f : ldexpf(l * f.fraction, f.power);
   const bool done = own == 1u;
   const PartialPlace part = done ? PartialPlace{nullptr, nullptr} : partial_place(a, item, local);
 #pragma unroll
@@ -594,7 +600,7 @@ __global__ __launch_bounds__((256 * kAttendOccupancy<C, ONE>), (kAttendOccupancy
     for (int c = 0; c < NR; ++c) {
       f32x4 o = chunk_value(s, round * NR + c, mid, r);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = l == 0.f ? 0.f : o[i] * f;
+      for (int i = 0; i < 4; ++i) o[i] = l == 0.f ? 0.f : ldexpf(o[i] * f.fraction, f.power);
       lds_o[wave][c][lane] = o;
     }
     __syncthreads();
