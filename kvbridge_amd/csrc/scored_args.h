@@ -29,6 +29,7 @@ struct ScoredArgs {
   uint32_t batch, rows, q_heads, kv_heads, group, head_rows, blocks;  // blocks of 16 head-rows per kv head
   uint32_t dim, page_tokens, pages, max_tokens, total_tokens, table_entries;
   uint32_t items, splits, split_tiles;  // work items per kv head and block, items per sequence (0: shared out), least tiles of one
+  uint32_t alone_tiles;  // up to so many tiles a sequence is not split
   uint32_t waves;  // of an attention work-group, at most (4, or all that a CU holds)
   uint32_t q_stride, q_type, out_type, window, kv_bits;
   float scale, cap;

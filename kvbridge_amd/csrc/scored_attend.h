@@ -322,17 +322,21 @@ template <int DIM, bool AGENT>
 __device__ __forceinline__ void merge_splits(const ScoredArgs& a, uint32_t b, uint32_t item0, uint32_t kv, uint32_t hr0,
                                              uint32_t count, uint32_t own, MergeLds& lds, uint32_t NT) {
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
+  constexpr uint32_t Q = DIM / 4, kAtOnce = 8;
+  const uint32_t items = count * Q;                     // (head-row, four dims)
+  const uint32_t groups = items < NT ? NT / items : 1u;  // of splits
+  const uint32_t ml_step = a.rows * a.q_heads * 2u;
+  const uint64_t step = uint64_t(a.rows) * a.q_heads * DIM;
   for (uint32_t r = wave; r < count; r += NT / 64u) {
     const float* ml = partial_place(a, item0, row_head(a, kv, hr0 + r)).ml;
-    const uint64_t step = uint64_t(a.rows) * a.q_heads * 2u;
     float top = neg_inf(), sum = 0.f;
-    for (uint32_t j = lane; j < own; j += 64u) top = fmaxf(top, load_pair(ml + step * j).x);
+    for (uint32_t j = lane; j < own; j += 64u) top = fmaxf(top, load_pair(ml + uint64_t(ml_step) * j).x);
     top = wave_max(top);
     for (uint32_t j = lane; j < own; j += 64u) {
-      const Pair p = load_pair(ml + step * j);
+      const Pair p = load_pair(ml + uint64_t(ml_step) * j);
       const float f = p.y == 0.f ? 0.f : exp_e(p.x - top);
       sum += p.y == 0.f ? 0.f : p.y * f;
-      if (j < kMergeSplits) lds.factor[r][j] = f;
+      lds.factor[r][j % kMergeSplits] = f;  // of the last 64 splits in the end
     }
     sum = wave_sum(sum);
     if (lane == 0u) {
@@ -340,20 +344,14 @@ __device__ __forceinline__ void merge_splits(const ScoredArgs& a, uint32_t b, ui
       lds.sum[r] = sum;
     }
   }
-  __syncthreads();
-  constexpr uint32_t Q = DIM / 4;
-  const uint32_t items = count * Q;                       // (head-row, four dims)
-  const uint32_t groups = items < NT ? NT / items : 1u;  // of splits
   for (uint32_t base = 0; base < items; base += NT) {
     const uint32_t item = groups > 1u ? tid % items : base + tid, group = groups > 1u ? tid / items : 0u;
     const bool in = item < items && group < groups;
-    const uint32_t r = in ? item / Q : 0u, quad = in ? item % Q : 0u;
-    const uint32_t local = row_head(a, kv, hr0 + r);
-    const uint64_t rh = uint64_t(b) * a.rows * a.q_heads + local, step = uint64_t(a.rows) * a.q_heads * DIM;
-    const float* o = partial_place(a, item0, local).o + 4u * quad;
+    const uint32_t r = in ? item / Q : 0u, local = row_head(a, kv, hr0 + r);
+    const float* o = partial_place(a, item0, local).o + 4u * (item % Q);
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     for (uint32_t c0 = 0; c0 < own; c0 += kMergeSplits) {
-      if (c0 > 0u || (base > 0u && own > kMergeSplits)) {  // the factors of these splits
+      if (own > kMergeSplits) {  // the factors of these splits
         __syncthreads();
         for (uint32_t i = tid; i < count * kMergeSplits; i += NT) {
           const uint32_t rr = i / kMergeSplits, j = c0 + i % kMergeSplits;
@@ -362,29 +360,29 @@ __device__ __forceinline__ void merge_splits(const ScoredArgs& a, uint32_t b, ui
             lds.factor[rr][i % kMergeSplits] = p.y == 0.f ? 0.f : exp_e(p.x - lds.top[rr]);
           }
         }
-        __syncthreads();
       }
+      __syncthreads();
       const uint32_t n = own - c0 < kMergeSplits ? own - c0 : kMergeSplits;
-      if (in) {
-        for (uint32_t j0 = group; j0 < n; j0 += 8u * groups) {
-          f32x4 x[8];
-          float f[8];
+      for (uint32_t j0 = group; in && j0 < n; j0 += kAtOnce * groups) {
+        f32x4 x[kAtOnce];
 #pragma unroll
-          for (uint32_t i = 0; i < 8u; ++i) {
-            const uint32_t j = j0 + i * groups, jc = j < n ? j : j0;
-            f[i] = j < n ? lds.factor[r][jc] : 0.f;
-            const float* p = o + (c0 + jc) * step;
-            if constexpr (AGENT) {
-              const Pair lo = load_pair(p), hi = load_pair(p + 2);
-              x[i] = f32x4{lo.x, lo.y, hi.x, hi.y};
-            } else {
-              x[i] = *reinterpret_cast<const f32x4*>(p);
-            }
+        for (uint32_t i = 0; i < kAtOnce; ++i) {
+          const uint32_t j = j0 + i * groups;
+          x[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+          if (j >= n) continue;
+          const float* p = o + (c0 + j) * step;
+          if constexpr (AGENT) {
+            const Pair lo = load_pair(p), hi = load_pair(p + 2);
+            x[i] = f32x4{lo.x, lo.y, hi.x, hi.y};
+          } else {
+            x[i] = *reinterpret_cast<const f32x4*>(p);
           }
+        }
 #pragma unroll
-          for (uint32_t i = 0; i < 8u; ++i) {
-            if (f[i] != 0.f) acc += x[i] * f[i];  // an empty split's are not written
-          }
+        for (uint32_t i = 0; i < kAtOnce; ++i) {
+          const uint32_t j = j0 + i * groups;
+          const float f = j < n ? lds.factor[r][j] : 0.f;
+          if (f != 0.f) acc += x[i] * f;  // an empty split's are not written
         }
       }
     }
@@ -395,10 +393,11 @@ __device__ __forceinline__ void merge_splits(const ScoredArgs& a, uint32_t b, ui
     }
     if (in && group == 0u) {
       const float sum = lds.sum[r];
+      const uint64_t rh = uint64_t(b) * a.rows * a.q_heads + local;
 #pragma unroll
       for (int k = 0; k < 4; ++k) acc[k] = sum == 0.f ? 0.f : acc[k] / sum;
-      store_out4(a, rh * a.dim + 4u * quad, acc);
-      if (quad == 0u) {
+      store_out4(a, rh * a.dim + 4u * (item % Q), acc);
+      if (item % Q == 0u) {
         a.m[rh] = sum == 0.f ? neg_inf() : lds.top[r];
         a.l[rh] = sum;
       }
@@ -477,12 +476,17 @@ __global__ __launch_bounds__((256 * kAttendOccupancy<C, ONE>), (kAttendOccupancy
   // next four Q, and by all the pages of the tiles that would be theirs if
   // positions count up from 0 to the last row's.
   const auto share = [&](const LiveTiles& t) {  // tiles of a split
-    const uint32_t per = t.n / it.count + (t.n % it.count != 0u ? 1u : 0u);
-    return per > a.split_tiles ? per : a.split_tiles;
+    uint32_t per = t.n / it.count + (t.n % it.count != 0u ? 1u : 0u);
+    per = per > a.split_tiles ? per : a.split_tiles;
+    return t.n <= a.alone_tiles ? a.alone_tiles : per;
   };
-  const auto tile_at = [&](const LiveTiles& t, uint32_t first, uint32_t i) {
-    const uint64_t x = uint64_t(first) + uint64_t(i) * NW;
-    return t.tile(x < t.n ? uint32_t(x) : t.n - 1u);
+  // The wave's i-th tile, from its last one backwards: with a bias by distance
+  // the largest scores come first, and the reference moves once instead of with
+  // every tile.
+  const auto tile_at = [&](const LiveTiles& t, uint32_t per, uint32_t i) {
+    const uint32_t first = split * per + wave, end = t.n - split * per > per ? split * per + per : t.n;
+    const uint32_t n = first < end ? (end - first - 1u) / NW : 0u, x = first + (i < n ? n - i : 0u) * NW;
+    return t.tile(x < t.n ? x : t.n - 1u);
   };
   const int64_t prefix = a.prefix ? a.prefix[b] : 0;
   const uint64_t behind = uint64_t(a.rows) - 1u + a.window;
@@ -490,8 +494,8 @@ __global__ __launch_bounds__((256 * kAttendOccupancy<C, ONE>), (kAttendOccupancy
                                       a.window != 0u && behind < e.tokens ? e.tokens - uint32_t(behind) : 0u, e.tokens);
   TilePages pages{0u, 0u};
   if (e.tokens > 0u) {
-    const uint32_t guess = split * share(likely) + wave;
-    pages = tile_pages(a, e, [&](uint32_t i) { return tile_at(likely, guess, i); }, 0u, lane);
+    const uint32_t guess = share(likely);
+    if (split * guess < likely.n) pages = tile_pages(a, e, [&](uint32_t i) { return tile_at(likely, guess, i); }, 0u, lane);
   }
   if (wave == 0u) {
     const int64_t qref = a.q_positions[uint64_t(b) * a.rows], qpos = a.q_positions[uint64_t(b) * a.rows + row];
@@ -546,11 +550,11 @@ __global__ __launch_bounds__((256 * kAttendOccupancy<C, ONE>), (kAttendOccupancy
   const uint32_t first = split * per + wave;
   const uint32_t end = live.n - split * per > per ? split * per + per : live.n;
   const uint32_t n = first < end ? (end - first + NW - 1u) / NW : 0u;
-  const auto tile_of = [&](uint32_t i) { return tile_at(live, first, i); };
+  const auto tile_of = [&](uint32_t i) { return tile_at(live, per, i); };
   uint32_t code_bits = 0x64006400u;
   asm("" : "+v"(code_bits));
   if (n > 0u) {
-    if (!live.same(likely)) pages = tile_pages(a, e, tile_of, 0u, lane);
+    if (!live.same(likely) || split * per >= likely.n) pages = tile_pages(a, e, tile_of, 0u, lane);
     TilePages ahead_pages = pages;
     TileRows<ONE> rows = tile_rows<ONE>(a, pages, 0u, kv);
     uint32_t t0 = tile_of(0u) * kTileTokens;

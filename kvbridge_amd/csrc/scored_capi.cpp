@@ -194,6 +194,7 @@ int kvb_decode_attention_scored(const kvb_scored_shape* s, const kvb_scored_inpu
     a.items = p.items;
     a.splits = p.splits;
     a.split_tiles = p.tiles;
+    a.alone_tiles = p.alone;
     a.waves = p.waves;
     a.scratch = scratch;
     a.counters = kvb::scored_one_launch(*s, p) ? counters : nullptr;

@@ -77,11 +77,13 @@ ScoredSplits split_items(const kvb_scored_shape& s, uint64_t others, uint32_t sp
     }
     const uint64_t splits = std::max<uint64_t>(1, (tiles + per - 1) / per);
     return ScoredSplits{uint32_t(std::min<uint64_t>(s.batch * splits, 0xffffffffu)), uint32_t(std::min<uint64_t>(splits, 0xffffffffu)),
-                        uint32_t(per), per < all ? 4u : waves};
+                        uint32_t(per), per < all ? 4u : waves, 0};
   }
-  const uint64_t least = 16, useful = s.batch * ((tiles + least - 1) / least);
+  // A tile costs a SIMD 0.8 us at dim 64 and 128 (twice that at 256), so a CU
+  // four of them; joining several parts costs about 3 us.
+  const uint64_t least = s.dim == 256 ? 4 : 8, useful = s.batch * ((tiles + least - 1) / least);
   const uint64_t items = std::max<uint64_t>(s.batch, std::min(useful, resident / others));
-  return ScoredSplits{uint32_t(items), s.batch == 1 ? uint32_t(items) : 0, uint32_t(least), waves};
+  return ScoredSplits{uint32_t(items), s.batch == 1 ? uint32_t(items) : 0, uint32_t(least), waves, s.dim == 256 ? 10u : 20u};
 }
 
 }  // namespace

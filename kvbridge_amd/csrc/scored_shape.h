@@ -20,6 +20,7 @@ struct ScoredSplits {
   uint32_t splits;  // items of every sequence; 0: the kernel shares them out by the sequences' lengths
   uint32_t tiles;   // least tiles of an item
   uint32_t waves;   // of a work-group
+  uint32_t alone;   // up to so many tiles a sequence is not split
 };
 ScoredSplits scored_splits(const kvb_scored_shape& s);
 // Whether the last work-group of a block merges its splits itself.
