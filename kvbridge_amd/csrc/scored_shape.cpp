@@ -92,13 +92,15 @@ ScoredSplits scored_splits(const kvb_scored_shape& s) {
   return split_items(s, uint64_t(s.kv_heads) * scored_blocks(s), s.split_tokens);
 }
 
-// One work-group's merge reads the partials of up to 16 head-rows past its L2,
-// eight splits of a thread's four dims a round: at most four rounds.  With 128
-// splits of 4 head-rows by 256 threads that took 14 us, a second launch over all
-// head-rows 5.
+// One work-group's merge reads the partials of its head-rows past its L2, a
+// second launch spreads that over a work-group per head-row.  Measured (us, one
+// launch against two) by the sets of four dims that a thread of the first has to
+// add: 1 (int8, window, 32 sequences) 111 / 114, 3 (16 ragged ones) 78.7 / 79.6,
+// 4 (four of 128K) 184 / 181, 5 (one of 64K) 27.7 / 24.8, 21 (24 heads of 256 over
+// 8 rows) 38.1 / 34.2.
 bool scored_one_launch(const kvb_scored_shape& s, const ScoredSplits& p) {
   const uint64_t head_rows = std::min<uint64_t>(16, uint64_t(s.rows) * (s.q_heads / s.kv_heads));
-  return p.items / s.batch * head_rows * (s.dim / 4) <= 32 * 64 * p.waves;
+  return p.items / s.batch * head_rows * (s.dim / 4) <= 3 * 64 * p.waves;
 }
 
 const char* scored_error(const kvb_scored_shape& s) {
