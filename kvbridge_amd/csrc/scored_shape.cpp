@@ -49,7 +49,8 @@ namespace {
 constexpr uint64_t kCus = 256;
 
 // Waves of the attention kernel that a CU holds (kAttendOccupancy in
-// scored_attend.h).
+// scored_attend.h).  One more wave per SIMD with spills inside the tile loop cost
+// a third to a half (16 ragged sequences 78 -> 160 us, 4 x 128K 186 -> 266).
 uint32_t resident_waves(const kvb_scored_shape& s) {
   const uint64_t head_rows = uint64_t(s.rows) * (s.q_heads / s.kv_heads), blocks = s.dim / 32;
   const bool half = s.kv_bits == 4 && s.dim > 64 && head_rows > 16 / blocks && head_rows <= 32 / blocks;
@@ -137,6 +138,10 @@ const char* evict_error(const kvb_evict_shape& s) {
   return nullptr;
 }
 
-ScoredSplits weight_splits(const kvb_scored_shape& s) { return split_items(s, s.kv_heads, 0); }
+ScoredSplits weight_splits(const kvb_scored_shape& s) {
+  ScoredSplits p = split_items(s, s.kv_heads, 0);
+  if (p.waves > 4) p.waves = 16;  // all that its work-group can have
+  return p;
+}
 
 }  // namespace kvb

@@ -14,9 +14,11 @@
 namespace kvb {
 namespace {
 
-// Waves per SIMD that the registers allow.
+// Waves per SIMD that the registers allow (at dim 64 four: 64 head-rows over int8
+// took 16 us with three, 11 with four; with a few spills outside the loop the
+// dim-128 kernels gained nothing).
 template <class C>
-constexpr int kWeightOccupancy = C::kGroups == 8 || (C::kF > 1 && C::kH > 1) ? 2 : 3;
+constexpr int kWeightOccupancy = C::kGroups == 8 || (C::kF > 1 && C::kH > 1) ? 2 : (C::kGroups == 2 && C::kF == 1 ? 4 : 3);
 
 __device__ __forceinline__ float row_sum16(float x) {
   x += row_ror<8>(x);
