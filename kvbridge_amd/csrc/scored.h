@@ -788,27 +788,29 @@ struct ScoreForm {
 __device__ __forceinline__ ScoreForm score_form(const ScoredArgs& a, float factor, float slope, int back) {
   return ScoreForm{factor, a.cap, a.cap > 0.f ? 1.f / a.cap : 0.f, slope, back};
 }
-template <class C>
-__device__ __forceinline__ void apply_form(const ScoredArgs& a, const ScoreForm& f, int ahead, uint32_t t0, uint32_t kg,
-                                           bool masked, uint32_t lo, uint32_t hi, uint32_t pre, float (&x)[8]) {
+// x: products of N of the tile's tokens, number(i) the lane's i-th one, far(i)
+// its position less that of the sequence's first row.
+template <int N, typename Number, typename Far>
+__device__ __forceinline__ void apply_form(const ScoredArgs& a, const ScoreForm& f, bool masked, uint32_t lo, uint32_t hi,
+                                           uint32_t pre, Number number, Far far, float (&x)[N]) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) x[j] *= f.factor;
+  for (int i = 0; i < N; ++i) x[i] *= f.factor;
   if (a.cap > 0.f) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = capped(x[j], f.cap, f.inv_cap);
+    for (int i = 0; i < N; ++i) x[i] = capped(x[i], f.cap, f.inv_cap);
   }
   if (a.slopes != nullptr) {
-    unrolled<0, 8>([&](auto jc) {
-      constexpr int j = jc;
-      x[j] = fmaf(f.slope, float(bci<j>(ahead) - f.back), x[j]);
-    });
+    int d[N];
+    far(d);
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = fmaf(f.slope, float(d[i] - f.back), x[i]);
   }
   if (masked) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t t = t0 + C::token(kg, j);
+    for (int i = 0; i < N; ++i) {
+      const uint32_t t = number(i);
       const bool seen = (t >= lo && t < hi) || t < pre;
-      x[j] = seen ? x[j] : neg_inf();
+      x[i] = seen ? x[i] : neg_inf();
     }
   }
 }

@@ -572,7 +572,8 @@ __global__ __launch_bounds__((256 * kAttendOccupancy<C, ONE>), (kAttendOccupancy
       float x[8];
       tile_scores<C, QD>(k, lds_q, lane, x);
       const bool whole = t0 + kTileTokens <= vis.pre || (t0 >= vis.all_lo && t0 + kTileTokens <= vis.all_hi);
-      apply_form<C>(a, form, ahead, t0, kg, !whole, vis.lo, vis.hi, vis.pre, x);
+      apply_form<8>(a, form, !whole, vis.lo, vis.hi, vis.pre, [&](int j) { return t0 + C::token(kg, j); },
+                    [&](int(&d)[8]) { unrolled<0, 8>([&](auto j) { d[j] = bci<j>(ahead); }); }, x);
       s.mtop = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])), s.mtop));
       keep_range(v, x, s);
       if (!whole) hide_odd_params(v, x, s, kg);

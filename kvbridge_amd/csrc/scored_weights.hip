@@ -7,8 +7,9 @@
 // slot) of a sequence is written by one wave only and in one order.  The
 // operands of as many blocks of 16 head-rows as fit 64 KiB of LDS are staged at
 // once and a tile's K serves all of them; more head-rows take another pass over
-// the item.  The sum over the head-rows of a block is a DPP reduction over the
-// 16 lanes of a row.
+// the item.  Where a head-row has F columns, whose lanes all hold its scores,
+// each of them goes on with 8 / F of the lane group's tokens; the sum over the
+// head-rows of a block is then a DPP reduction over every F-th lane of a row.
 #include "scored.h"
 
 namespace kvb {
@@ -20,12 +21,25 @@ namespace {
 template <class C>
 constexpr int kWeightOccupancy = C::kGroups == 8 || (C::kF > 1 && C::kH > 1) ? 2 : (C::kGroups == 2 && C::kF == 1 ? 4 : 3);
 
-__device__ __forceinline__ float row_sum16(float x) {
+// Sum over the lanes r % F of a row.
+template <int F>
+__device__ __forceinline__ float rows_of_f_sum(float x) {
   x += row_ror<8>(x);
-  x += row_ror<4>(x);
-  x += row_ror<2>(x);
-  x += row_ror<1>(x);
+  if constexpr (F <= 4) x += row_ror<4>(x);
+  if constexpr (F <= 2) x += row_ror<2>(x);
+  if constexpr (F <= 1) x += row_ror<1>(x);
   return x;
+}
+// Of eight values the N = 8 / F from f * N on.
+template <int F, typename T>
+__device__ __forceinline__ void share_of(const T (&x)[8], uint32_t f, T (&y)[8 / F]) {
+  constexpr int N = 8 / F;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    y[i] = x[i];
+#pragma unroll
+    for (int k = 1; k < F; ++k) y[i] = f == uint32_t(k) ? x[k * N + i] : y[i];
+  }
 }
 
 // A block's head-rows next to their Q operands.
@@ -44,9 +58,10 @@ __global__ __launch_bounds__((256 * kWeightOccupancy<C>), (kWeightOccupancy<C>))
   extern __shared__ __align__(16) uint8_t lds_raw[];
   using Block = WeightBlock<C, QD>;
   Block* const blocks = reinterpret_cast<Block*>(lds_raw);
+  constexpr int F = C::kF, N = 8 / F;
   __shared__ WorkItem plan_it;
-  __shared__ uint32_t plan_found, plan_pre, plan_lo, plan_hi;
-  const uint32_t lane = threadIdx.x & 63u, r = lane & 15u, kg = lane >> 4, NW = blockDim.x >> 6;
+  __shared__ uint32_t plan_found, plan_pre, plan_lo, plan_hi, plan_all_lo, plan_all_hi;
+  const uint32_t lane = threadIdx.x & 63u, r = lane & 15u, f = r % F, kg = lane >> 4, NW = blockDim.x >> 6;
   const uint32_t wave = uniform(threadIdx.x >> 6);
   const uint32_t kv = blockIdx.x % a.kv_heads, item = blockIdx.x / a.kv_heads;
   if (wave == 0u) {
@@ -72,9 +87,10 @@ __global__ __launch_bounds__((256 * kWeightOccupancy<C>), (kWeightOccupancy<C>))
     return per > a.split_tiles ? per : a.split_tiles;
   };
 
-  // The tokens that any row sees, by the last wave: one row per lane.
+  // The tokens that any row sees and those that all see, by the last wave: one
+  // row per lane.
   if (wave == NW - 1u) {
-    uint32_t lo = 0xffffffffu, hi = 0u, pre = 0u;
+    uint32_t lo = 0xffffffffu, hi = 0u, pre = 0u, all_lo = 0u, all_hi = 0xffffffffu;
     for (uint32_t row0 = 0; row0 < a.rows; row0 += 64u) {
       const bool valid = row0 + lane < a.rows;
       const Visible v = visible_tokens(a, e, valid, ask_visible(a, e, q_positions[valid ? row0 + lane : 0u], prefix));
@@ -82,10 +98,17 @@ __global__ __launch_bounds__((256 * kWeightOccupancy<C>), (kWeightOccupancy<C>))
         lo = v.lo < lo ? v.lo : lo;
         hi = v.hi > hi ? v.hi : hi;
       }
+      if (valid) {
+        all_lo = v.lo > all_lo ? v.lo : all_lo;
+        all_hi = v.hi < all_hi ? v.hi : all_hi;
+      }
       pre = v.pre;
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
+      const uint32_t l3 = uint32_t(__shfl_xor(int(all_lo), o)), h3 = uint32_t(__shfl_xor(int(all_hi), o));
+      all_lo = l3 > all_lo ? l3 : all_lo;
+      all_hi = h3 < all_hi ? h3 : all_hi;
       const uint32_t l2 = uint32_t(__shfl_xor(int(lo), o)), h2 = uint32_t(__shfl_xor(int(hi), o));
       lo = l2 < lo ? l2 : lo;
       hi = h2 > hi ? h2 : hi;
@@ -94,6 +117,8 @@ __global__ __launch_bounds__((256 * kWeightOccupancy<C>), (kWeightOccupancy<C>))
       plan_pre = pre;
       plan_lo = hi == 0u ? 0u : lo;
       plan_hi = hi;
+      plan_all_lo = all_lo;
+      plan_all_hi = all_hi;
     }
   }
 
@@ -124,13 +149,13 @@ __global__ __launch_bounds__((256 * kWeightOccupancy<C>), (kWeightOccupancy<C>))
         w.lo[r] = vis.lo;
         w.hi[r] = vis.hi;
         w.m[r] = counts ? m : FLT_MAX;
-        w.per_l[r] = counts && r % C::kF == 0u ? 1.f / l : 0.f;  // a head-row's F columns hold the same score
+        w.per_l[r] = counts ? 1.f / l : 0.f;
         w.slope[r] = a.slopes ? a.slopes[head] : 0.f;
         w.back[r] = near(int64_t(uint64_t(qpos) - uint64_t(qref)));
       }
     }
     __syncthreads();
-    const uint32_t pre = uniform(plan_pre);
+    const uint32_t pre = uniform(plan_pre), all_lo = uniform(plan_all_lo), all_hi = uniform(plan_all_hi);
     const LiveTiles live = live_tiles(pre, uniform(plan_lo), uniform(plan_hi));
     const uint32_t per = share(live.n);
     const uint32_t t_first = split * per + wave;
@@ -153,24 +178,35 @@ __global__ __launch_bounds__((256 * kWeightOccupancy<C>), (kWeightOccupancy<C>))
         const TileRows<ONE> rows_next = tile_rows<ONE>(a, pages, i + 1u < n ? i + 1u : i, kv);
         const typename C::K k_next = C::template load_k<ONE>(a, rows_next, r, kg, e.tokens - t_next);
         const int ahead_next = load_ahead<C>(a, e, t_next, r, kg, qref);
-        float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        const bool whole = t0 + kTileTokens <= pre || (t0 >= all_lo && t0 + kTileTokens <= all_hi);
+        float sum[N];
+#pragma unroll
+        for (int i2 = 0; i2 < N; ++i2) sum[i2] = 0.f;
         for (uint32_t bl = 0; bl < count; ++bl) {
           asm volatile("" ::: "memory");  // the operands stay in LDS: not hoisted out of the loops
           const Block& w = blocks[bl];
-          float x[8];
+          float x[8], y[N];
           tile_scores<C, QD>(k, w.q, lane, x);
+          share_of<F>(x, f, y);
           const ScoreForm form = score_form(a, w.q.factor[r], w.slope[r], w.back[r]);
-          apply_form<C>(a, form, ahead, t0, kg, true, w.lo[r], w.hi[r], pre, x);
+          apply_form<N>(a, form, !whole, w.lo[r], w.hi[r], pre, [&](int j) { return t0 + C::token(kg, f * N + j); },
+                        [&](int(&d)[N]) {
+                          int all[8];
+                          unrolled<0, 8>([&](auto j) { all[j] = bci<j>(ahead); });
+                          share_of<F>(all, f, d);
+                        },
+                        y);
           const float m = w.m[r], per_l = w.per_l[r];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) sum[j] = fmaf(per_l > 0.f ? exp_e(x[j] - m) : 0.f, per_l, sum[j]);
+          for (int i2 = 0; i2 < N; ++i2) sum[i2] = fmaf(exp_e(y[i2] - m), per_l, sum[i2]);
         }
-        float total = row_sum16(sum[0]);
-        unrolled<1, 8>([&](auto jc) {
-          const float s = row_sum16(sum[jc]);
-          total = r == uint32_t(jc) ? s : total;
+        // Lane i F + f of the row's first eight writes its lanes' token i.
+        float total = rows_of_f_sum<F>(sum[0]);
+        unrolled<1, N>([&](auto jc) {
+          const float s = rows_of_f_sum<F>(sum[jc]);
+          total = r / F == uint32_t(jc) ? s : total;
         });
-        const uint32_t in = C::token(kg, r % 8u), tok = t0 + in;
+        const uint32_t in = C::token(kg, f * N + r % 8u / F), tok = t0 + in;
         if (r < 8u && tok < e.tokens) {
           const uint32_t P = a.page_tokens;
           const uint64_t at = ONE ? rows.row(0, P) + in
