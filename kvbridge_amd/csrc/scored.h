@@ -57,7 +57,7 @@ typedef uint32_t u32x4_s __attribute__((ext_vector_type(4)));
 
 constexpr uint32_t kTileTokens = 32;
 
-// Lane J of each 16-lane row, for folding into the using instruction.  Every
+// Lane J of each 16-lane row.  Every
 // lane must be active where it is called: outside of selects and branches.
 template <int J>
 __device__ __forceinline__ float bc(float x) {
@@ -66,6 +66,63 @@ __device__ __forceinline__ float bc(float x) {
 template <int J>
 __device__ __forceinline__ int bci(int x) {
   return __builtin_amdgcn_mov_dpp(x, 0x150 + J, 0xF, 0xF, true);
+}
+
+// For a lane group's eight tokens, whose parameters of one block lie in lanes L,
+// L + 2, .. of its row: x[j] += step_j d_j + least_j sum, d_j products of the
+// matrix unit.  The compiler gives every broadcast into a fused multiply-add a
+// v_mov_b32 of its own (with weigh_block 1,114 -> 858 vector instructions per
+// tile at dim 256, f32; two sequences of 32K under 16 head-rows of dim 128 38.2
+// -> 35.3 us).  The waits inside are the author's: 2 states from a write to a
+// DPP read, 19 from the longest matrix product to a read of its result (2 + 8 +
+// 12 here).
+template <int L>
+__device__ __forceinline__ void add_block(float (&x)[8], float step, float least, const f32x4& da, const f32x4& db, float sum) {
+  asm("s_nop 1\n\t"
+      "v_fmac_f32_dpp %0, %9, %10 row_newbcast:%c19 row_mask:0xf bank_mask:0xf\n\t"
+      "v_fmac_f32_dpp %1, %9, %10 row_newbcast:%c20 row_mask:0xf bank_mask:0xf\n\t"
+      "v_fmac_f32_dpp %2, %9, %10 row_newbcast:%c21 row_mask:0xf bank_mask:0xf\n\t"
+      "v_fmac_f32_dpp %3, %9, %10 row_newbcast:%c22 row_mask:0xf bank_mask:0xf\n\t"
+      "v_fmac_f32_dpp %4, %9, %10 row_newbcast:%c23 row_mask:0xf bank_mask:0xf\n\t"
+      "v_fmac_f32_dpp %5, %9, %10 row_newbcast:%c24 row_mask:0xf bank_mask:0xf\n\t"
+      "v_fmac_f32_dpp %6, %9, %10 row_newbcast:%c25 row_mask:0xf bank_mask:0xf\n\t"
+      "v_fmac_f32_dpp %7, %9, %10 row_newbcast:%c26 row_mask:0xf bank_mask:0xf\n\t"
+      "s_nop 11\n\t"
+      "v_fmac_f32_dpp %0, %8, %11 row_newbcast:%c19 row_mask:0xf bank_mask:0xf\n\t"
+      "v_fmac_f32_dpp %1, %8, %12 row_newbcast:%c20 row_mask:0xf bank_mask:0xf\n\t"
+      "v_fmac_f32_dpp %2, %8, %13 row_newbcast:%c21 row_mask:0xf bank_mask:0xf\n\t"
+      "v_fmac_f32_dpp %3, %8, %14 row_newbcast:%c22 row_mask:0xf bank_mask:0xf\n\t"
+      "v_fmac_f32_dpp %4, %8, %15 row_newbcast:%c23 row_mask:0xf bank_mask:0xf\n\t"
+      "v_fmac_f32_dpp %5, %8, %16 row_newbcast:%c24 row_mask:0xf bank_mask:0xf\n\t"
+      "v_fmac_f32_dpp %6, %8, %17 row_newbcast:%c25 row_mask:0xf bank_mask:0xf\n\t"
+      "v_fmac_f32_dpp %7, %8, %18 row_newbcast:%c26 row_mask:0xf bank_mask:0xf"
+      : "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3]), "+v"(x[4]), "+v"(x[5]), "+v"(x[6]), "+v"(x[7])
+      : "v"(step), "v"(least), "v"(sum), "v"(da[0]), "v"(da[1]), "v"(da[2]), "v"(da[3]), "v"(db[0]), "v"(db[1]), "v"(db[2]),
+        "v"(db[3]), "n"(L), "n"(L + 2), "n"(L + 4), "n"(L + 6), "n"(L + 8), "n"(L + 10), "n"(L + 12), "n"(L + 14));
+}
+// The same for weights p: w[j] = step_j p_j, mid += at8_j p_j.
+template <int L>
+__device__ __forceinline__ void weigh_block(float (&w)[8], float& mid, float step, float at8, const float (&p)[8]) {
+  asm("s_nop 1\n\t"
+      "v_mul_f32_dpp %0, %9, %11 row_newbcast:%c19 row_mask:0xf bank_mask:0xf\n\t"
+      "v_mul_f32_dpp %1, %9, %12 row_newbcast:%c20 row_mask:0xf bank_mask:0xf\n\t"
+      "v_mul_f32_dpp %2, %9, %13 row_newbcast:%c21 row_mask:0xf bank_mask:0xf\n\t"
+      "v_mul_f32_dpp %3, %9, %14 row_newbcast:%c22 row_mask:0xf bank_mask:0xf\n\t"
+      "v_mul_f32_dpp %4, %9, %15 row_newbcast:%c23 row_mask:0xf bank_mask:0xf\n\t"
+      "v_mul_f32_dpp %5, %9, %16 row_newbcast:%c24 row_mask:0xf bank_mask:0xf\n\t"
+      "v_mul_f32_dpp %6, %9, %17 row_newbcast:%c25 row_mask:0xf bank_mask:0xf\n\t"
+      "v_mul_f32_dpp %7, %9, %18 row_newbcast:%c26 row_mask:0xf bank_mask:0xf\n\t"
+      "v_fmac_f32_dpp %8, %10, %11 row_newbcast:%c19 row_mask:0xf bank_mask:0xf\n\t"
+      "v_fmac_f32_dpp %8, %10, %12 row_newbcast:%c20 row_mask:0xf bank_mask:0xf\n\t"
+      "v_fmac_f32_dpp %8, %10, %13 row_newbcast:%c21 row_mask:0xf bank_mask:0xf\n\t"
+      "v_fmac_f32_dpp %8, %10, %14 row_newbcast:%c22 row_mask:0xf bank_mask:0xf\n\t"
+      "v_fmac_f32_dpp %8, %10, %15 row_newbcast:%c23 row_mask:0xf bank_mask:0xf\n\t"
+      "v_fmac_f32_dpp %8, %10, %16 row_newbcast:%c24 row_mask:0xf bank_mask:0xf\n\t"
+      "v_fmac_f32_dpp %8, %10, %17 row_newbcast:%c25 row_mask:0xf bank_mask:0xf\n\t"
+      "v_fmac_f32_dpp %8, %10, %18 row_newbcast:%c26 row_mask:0xf bank_mask:0xf"
+      : "=&v"(w[0]), "=&v"(w[1]), "=&v"(w[2]), "=&v"(w[3]), "=&v"(w[4]), "=&v"(w[5]), "=&v"(w[6]), "=&v"(w[7]), "+v"(mid)
+      : "v"(step), "v"(at8), "v"(p[0]), "v"(p[1]), "v"(p[2]), "v"(p[3]), "v"(p[4]), "v"(p[5]), "v"(p[6]), "v"(p[7]), "n"(L),
+        "n"(L + 2), "n"(L + 4), "n"(L + 6), "n"(L + 8), "n"(L + 10), "n"(L + 12), "n"(L + 14));
 }
 
 __device__ __forceinline__ uint32_t uniform(uint32_t x) { return uint32_t(__builtin_amdgcn_readfirstlane(int(x))); }
@@ -731,12 +788,17 @@ __device__ __forceinline__ void tile_scores(const typename C::K& k, const QBlock
         }
       });
       const float sum = q.sum[h][lane % 16u];
-      unrolled<0, 8>([&](auto jc) {
-        constexpr int j = jc;
-        const float d = j < 4 ? da[j % 4] : db[j % 4];
-        x[j] = fmaf(p.template step_of<j, h>(), d, x[j]);
-        x[j] = fmaf(p.template other_of<j, h>(), sum, x[j]);
-      });
+      if constexpr (F == 1) {
+        constexpr int PW = C::kPWords;
+        add_block<h / PW>(x, p.step[h % PW], p.other[h % PW], da, db, sum);
+      } else {
+        unrolled<0, 8>([&](auto jc) {
+          constexpr int j = jc;
+          const float d = j < 4 ? da[j % 4] : db[j % 4];
+          x[j] = fmaf(p.template step_of<j, h>(), d, x[j]);
+          x[j] = fmaf(p.template other_of<j, h>(), sum, x[j]);
+        });
+      }
     });
 #pragma unroll
     for (int j = 0; j < 8; ++j) x[j] = lanes_sum<F>(x[j]);

@@ -131,15 +131,31 @@ template <int PD>
 struct PDigits {
   f16x8 d[PD];
 };
+// w less an fp16 (the low or high half of a dword) in one instruction; the
+// compiler converts first and subtracts then.
+template <int HALF>
+__device__ __forceinline__ float less_half(float w, uint32_t halves) {
+  float r;
+  if constexpr (HALF == 0) asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(halves), "v"(w));
+  else asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(halves), "v"(w));
+  return r;
+}
 template <int PD>
 __device__ __forceinline__ PDigits<PD> p_digits(const float (&w)[8]) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+  uint32_t d[PD][4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float a = w[2 * j], b = w[2 * j + 1];
+    d[0][j] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), f16x2));
+    if constexpr (PD == 2)
+      d[1][j] = __builtin_bit_cast(
+          uint32_t, __builtin_convertvector((f32x2{less_half<0>(a, d[0][j]), less_half<1>(b, d[0][j])}), f16x2));
+  }
   PDigits<PD> p;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const _Float16 hi = _Float16(w[j]);
-    p.d[0][j] = hi;
-    if constexpr (PD == 2) p.d[1][j] = _Float16(w[j] - float(hi));
-  }
+  for (int i = 0; i < PD; ++i) p.d[i] = as_f16x8(d[i][0], d[i][1], d[i][2], d[i][3]);
   return p;
 }
 
@@ -227,12 +243,17 @@ __device__ __forceinline__ void tile_values(const typename Cache4<G, F>::V& v, c
   unrolled<0, C::kH>([&](auto hc) {
     constexpr int h = hc;
     float w[8];
-    unrolled<0, 8>([&](auto jc) {
-      constexpr int j = jc;
-      const float step = par.template step_of<j, h>(), at8 = par.template other_of<j, h>();
-      w[j] = step * p[j];
-      s.mid[h] = fmaf(at8, p[j], s.mid[h]);
-    });
+    if constexpr (F == 1) {
+      constexpr int PW = C::kPWords;
+      weigh_block<h / PW>(w, s.mid[h], par.step[h % PW], par.other[h % PW], p);
+    } else {
+      unrolled<0, 8>([&](auto jc) {
+        constexpr int j = jc;
+        const float step = par.template step_of<j, h>(), at8 = par.template other_of<j, h>();
+        w[j] = step * p[j];
+        s.mid[h] = fmaf(at8, p[j], s.mid[h]);
+      });
+    }
     const PDigits<PD> d = p_digits<PD>(w);
     unrolled<0, F>([&](auto fc) {
       constexpr int g = fc * C::kH + h;
