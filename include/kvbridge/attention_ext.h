@@ -10,7 +10,7 @@
 namespace kvbridge {
 
 // Output element type of the normalize step.
-enum class OutputType : int { none = 0, f32 = 1, f16 = 2 };
+enum class OutputType : int { none = 0, f32 = 1, f16 = 2, bf16 = 3 };  // bf16: the calls on a 4- or 8-bit cache below
 
 // Splits over [begin, end) when each split covers split_tokens tokens
 // (max(1, ceil((end - begin) / split_tokens))).  Validates the shape first;
@@ -109,5 +109,94 @@ struct AppendShape {
 // std::runtime_error for a launch failure.  Asynchronous on `stream`.
 void append_kv(const AppendShape&, const void* k_new, const void* v_new, const uint32_t* slots, int8_t* k,
                int8_t* v, float* k_scales, float* v_scales, hipStream_t stream);
+
+// ---- 4-bit cache, score forms and eviction.  Formats, formulas, buffers and
+// what the calls may share: include/kvbridge_c.h.  Every call throws
+// std::invalid_argument for an invalid shape or buffer before anything is
+// enqueued, std::runtime_error for a launch failure, and is asynchronous on
+// `stream`; the *_error functions return nullptr when valid and never throw.
+
+// Quantizes new tokens' rows into their slots of a 4-bit pool (blocks of 32
+// dims, bfloat16 step and least value).  The shape is append_kv's.
+const char* append_i4_error(const AppendShape&) noexcept;
+void append_kv_i4(const AppendShape&, const void* k_new, const void* v_new, const uint32_t* slots, uint8_t* k,
+                  uint8_t* v, uint32_t* k_scales, uint32_t* v_scales, hipStream_t stream);
+
+// The rows of `slots` as values, k_out / v_out[(t * kv_heads + kv) * dim + d].
+struct ReadShape {
+  unsigned tokens, kv_heads, dim, page_tokens, pages;
+  unsigned kv_bits;  // 4 or 8
+  OutputType out_type;
+};
+const char* read_shape_error(const ReadShape&) noexcept;
+void read_kv(const ReadShape&, const uint32_t* slots, const void* k, const void* v, const void* k_scales,
+             const void* v_scales, void* k_out, void* v_out, hipStream_t stream);
+
+// Ragged decode attention under score forms: tanh cap, bias by distance, window,
+// prefix.
+struct ScoredShape {
+  unsigned batch, rows, q_heads, kv_heads, dim, page_tokens, pages;
+  unsigned max_tokens, total_tokens, table_entries;  // as BatchShape
+  unsigned split_tokens;  // a multiple of 32, or 0: the library's choice
+  unsigned kv_bits;       // 4 or 8
+  SourceType q_type;
+  unsigned q_stride;      // elements from one query row to the next
+  unsigned window;        // 0: none
+  float scale, cap;       // cap 0: none
+};
+struct ScoredInput {
+  const void* q;                // [batch][rows][q_stride]
+  const int64_t* q_positions;   // [batch][rows]
+  const uint32_t* seq_starts;   // [batch + 1]
+  const uint32_t* page_offsets; // [batch]
+  const int64_t* k_positions;   // [total_tokens]
+  const uint32_t* page_table;   // [table_entries]
+  const void* k;
+  const void* v;
+  const void* k_scales;
+  const void* v_scales;
+  const float* slopes;          // [q_heads] or nullptr
+  const int64_t* prefix;        // [batch] or nullptr
+};
+const char* scored_shape_error(const ScoredShape&) noexcept;
+unsigned scored_item_count(const ScoredShape&);       // validate
+size_t scored_scratch_elements(const ScoredShape&);   // floats
+size_t scored_counter_elements(const ScoredShape&);   // uint32, zero before the first call and left zero
+void decode_attention_scored(const ScoredShape&, const ScoredInput&, float* scratch, uint32_t* counters, float* m,
+                             float* l, void* out, OutputType out_type, hipStream_t stream);
+
+// weights[(page * kv_heads + kv) * page_tokens + slot] += the token's share of
+// the attention with these m and l; the last `fresh` tokens are set.
+void accumulate_weights(const ScoredShape&, const ScoredInput&, const float* m, const float* l, unsigned fresh,
+                        float* weights, hipStream_t stream);
+
+// Which tokens stay (select), and packing them into other pages (move).
+struct EvictShape {
+  unsigned batch, kv_heads, dim, page_tokens, pages;
+  unsigned max_tokens, total_tokens, table_entries, dst_entries;
+  unsigned keep, sink, recent, kv_bits;
+};
+struct EvictInput {
+  const uint32_t* seq_starts;
+  const uint32_t* page_offsets;
+  const uint32_t* page_table;
+  const int64_t* k_positions;  // nullptr where no positions are moved
+};
+struct EvictCache {
+  void* k;
+  void* v;
+  void* k_scales;
+  void* v_scales;
+  float* weights;               // or nullptr
+  const uint32_t* dst_offsets;  // [batch]
+  const uint32_t* dst_table;    // [dst_entries]
+  int64_t* positions;           // [batch * keep] or nullptr
+};
+const char* evict_shape_error(const EvictShape&) noexcept;
+size_t evict_scratch_elements(const EvictShape&);  // uint32
+void evict_select(const EvictShape&, const EvictInput&, const float* weights, uint32_t* scratch, uint32_t* kept,
+                  uint32_t* kept_starts, hipStream_t stream);
+void evict_move(const EvictShape&, const EvictInput&, const EvictCache&, const uint32_t* kept,
+                const uint32_t* kept_starts, hipStream_t stream);
 
 }  // namespace kvbridge

@@ -272,19 +272,23 @@ int kvb_read_kv(const kvb_read_shape* s, const kvb_read_io* io, void* stream);
  *   t is visible when k_position <= q_position and (window == 0 or q_position -
  *   k_position < window), or when prefix != NULL and k_position < prefix[b].
  * m = max s, l = sum exp(s - m), out = sum exp(s - m) v / l over the visible
- * tokens; m = -inf, l = 0, out = 0 where there is none.  What masked tokens
- * hold, NaN included, has no effect.  Distances of 2^30 and more count as 2^30.
- * k_positions are nondecreasing within a sequence.
+ * tokens; m = -inf, l = 0, out = 0 where there is none, or every s is -inf.
+ * What masked tokens hold, NaN included, has no effect; in a visible token a
+ * K scale or parameter that is not finite makes the row NaN, one of V the dims
+ * that it enters, if the token's weight is not 0 in fp32.  Distances of 2^30
+ * and more count as 2^30.  k_positions are nondecreasing within a sequence.
  * q is [batch][rows][q_heads][dim] of q_type (KVB_SRC_*) with q_stride elements
- * from one row to the next.  split_tokens is a multiple of 32, or 0 for the
- * library's choice.  Q of fp32 enters the products as two fp16 digits, the
- * weights as one (out bf16 from 16-bit q) or two, each scaled by a power of two
- * per row, and every sum is fp32.
- * Buffers: kvb_scored_scratch_elements floats; m, l [batch][rows][q_heads];
- * out [batch][rows][q_heads][dim] in out_type (KVB_OUT_F32, _F16 or _BF16);
- * counters: NULL (a second launch merges the splits), or
- * kvb_scored_counter_elements uint32, zero before the first call and left zero
- * (one launch).  Calls that share scratch or counters must not overlap. */
+ * from one row to the next.  split_tokens is a multiple of 32, or 0: up to 256
+ * sequences then get items by their lengths, read on the device.  Q enters the
+ * products as one fp16 digit (kv_bits 8, 16-bit q) or two, the weights as one
+ * (out bf16 from 16-bit q) or two, each scaled by a power of two per row, and
+ * every sum is fp32.
+ * Buffers: kvb_scored_scratch_elements floats and out 16-byte aligned; m, l
+ * [batch][rows][q_heads]; out [batch][rows][q_heads][dim] in out_type
+ * (KVB_OUT_F32, _F16 or _BF16); counters: NULL (a second launch merges the
+ * items), or kvb_scored_counter_elements uint32, zero before the first call and
+ * left zero (the merge runs in the same launch where it is short).  Calls that
+ * share scratch or counters, graph replays included, must not overlap. */
 typedef struct kvb_scored_shape {
   uint32_t batch, rows, q_heads, kv_heads, dim, page_tokens, pages;
   uint32_t max_tokens, total_tokens, table_entries, split_tokens;
@@ -321,7 +325,8 @@ int kvb_decode_attention_scored(const kvb_scored_shape* s, const kvb_scored_inpu
  * masked or l is 0.  The last `fresh` tokens of each sequence (those that no
  * earlier call has counted) are set to that sum instead of added to.  The
  * adding is atomic: a page in several sequences gets every sequence's sum, in
- * any order; a page in one sequence gives the same bits in every run. */
+ * any order; a page in one sequence gives the same bits in every run.  A token
+ * that several sequences share must be fresh in none of them. */
 int kvb_accumulate_weights(const kvb_scored_shape* s, const kvb_scored_input* in, const float* m, const float* l,
                            uint32_t fresh, float* weights, void* stream);
 
@@ -331,12 +336,13 @@ int kvb_accumulate_weights(const kvb_scored_shape* s, const kvb_scored_input* in
  * least; equal ones: the earlier token).  kvb_evict_select writes their logical
  * indices, ascending, to kept[b * keep ..] (entries past the count are left as
  * they are), and kept_starts[b] = tokens kept before sequence b, [batch + 1].
- * scratch: kvb_evict_scratch_elements uint32.
+ * scratch: kvb_evict_scratch_elements uint32, 16-byte aligned.  k_positions is
+ * read by the move alone, and only where positions are given.
  * kvb_evict_move packs the kept tokens into other pages of the same pool: logical
  * token j of sequence b in the destination is slot j % page_tokens of page
  * dst_table[dst_offsets[b] + j / page_tokens], and gets codes, scales, the
- * weight (weights may be NULL) and the position (positions[kept_starts[b] + j],
- * may be NULL) of token kept[b * keep + j].  kept_starts and positions are then
+ * weight (weights may be NULL) and the position (positions[kept_starts[b] + j] of
+ * batch * keep, may be NULL) of token kept[b * keep + j].  kept_starts and positions are then
  * seq_starts and k_positions of the next call.  A destination page must not be
  * a page that this call reads, nor occur twice.  Ids >= pages are skipped. */
 typedef struct kvb_evict_shape {

@@ -196,7 +196,7 @@ __global__ __launch_bounds__(256) void read4_kernel(const ReadArgs a) {
 template <class T, int G>
 __global__ __launch_bounds__(256) void read8_kernel(const ReadArgs a) {
   constexpr uint32_t D = 32u * G, W = D + 8u;  // LDS row: 16-byte pieces, rows two banks apart
-  __shared__ uint8_t tile[64 * W];
+  __shared__ __align__(16) uint8_t tile[64 * W];
   __shared__ uint32_t pages[64], slots[64];
   const uint32_t kv = blockIdx.y, t0 = blockIdx.x * 64u;
   const bool is_v = blockIdx.z != 0u;
@@ -222,11 +222,10 @@ __global__ __launch_bounds__(256) void read8_kernel(const ReadArgs a) {
     if (pages[t] < a.pages) {
       const uint64_t row = (uint64_t(pages[t]) * a.kv_heads + kv) * a.page_tokens + slots[t];
       const float scale = static_cast<const float*>(is_v ? a.v_scales : a.k_scales)[row];
-      uint8_t c[8];
-      *reinterpret_cast<u32x2_c*>(c) = is_v ? *reinterpret_cast<const u32x2_c*>(tile + t * W + d)
-                                            : *reinterpret_cast<const u32x2_c*>(static_cast<const uint8_t*>(a.k) + row * D + d);
+      const u32x2_c c = is_v ? *reinterpret_cast<const u32x2_c*>(tile + t * W + d)
+                             : *reinterpret_cast<const u32x2_c*>(static_cast<const uint8_t*>(a.k) + row * D + d);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = float(int8_t(c[j])) * scale;
+      for (int j = 0; j < 8; ++j) x[j] = float(int8_t(c[j / 4] >> (8 * (j % 4)))) * scale;
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[j] = 0.f;
@@ -280,6 +279,11 @@ hipError_t launch_read(const ReadArgs& a, hipStream_t stream) {
   if (a.out_type == 1u) return read_type<float>(a, stream);
   if (a.out_type == 2u) return read_type<_Float16>(a, stream);
   return read_type<__bf16>(a, stream);
+}
+
+hipError_t preload_cache4() {
+  hipFuncAttributes attr;
+  return hipFuncGetAttributes(&attr, reinterpret_cast<const void*>(&append4_kernel<float, 2, true>));
 }
 
 }  // namespace kvb

@@ -17,6 +17,7 @@
 
 #include "kernels.h"
 #include "kvbridge/attention_ext.h"
+#include "scored_args.h"
 
 namespace {
 
@@ -278,6 +279,7 @@ int kvb_preload_attention_reference_kernels(void) {
   if (e == hipSuccess) e = kvb::preload_lds();
   if (e == hipSuccess) e = kvb::preload_merge();
   if (e == hipSuccess) e = kvb::preload_append();
+  if (e == hipSuccess) e = kvb::preload_scored();
   return int(e);
 }
 

@@ -361,4 +361,9 @@ hipError_t launch_evict_move(const EvictArgs& a, hipStream_t stream) {
   return hipGetLastError();
 }
 
+hipError_t preload_evict() {
+  hipFuncAttributes attr;
+  return hipFuncGetAttributes(&attr, reinterpret_cast<const void*>(&evict_keys_kernel));
+}
+
 }  // namespace kvb

@@ -195,7 +195,7 @@ __device__ __forceinline__ ItemShares item_shares(const ScoredArgs& a) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint32_t b = 64u * i + lane;
-      const uint32_t c = uint32_t(tiles[i] * per + 0.9990234375f);
+      const uint32_t c = uint32_t(fmaf(tiles[i], per, 0.9990234375f));  // one rounding in every kernel
       s.count[i] = b < a.batch ? (c > 1u ? c : 1u) : 0u;
       n += s.count[i];
     }

@@ -37,6 +37,12 @@ struct ScoredArgs {
   uint32_t fresh;
 };
 
+// Load the code objects of all these calls.
+hipError_t preload_scored();
+hipError_t preload_scored_weights();
+hipError_t preload_cache4();
+hipError_t preload_evict();
+
 hipError_t launch_scored_attend(const ScoredArgs& a, hipStream_t stream);
 hipError_t launch_scored_weights(const ScoredArgs& a, hipStream_t stream);
 

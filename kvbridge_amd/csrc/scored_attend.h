@@ -695,8 +695,8 @@ inline hipError_t launch_attend_kernel(const ScoredArgs& a, hipStream_t stream) 
   const bool one = a.page_tokens % kTileTokens == 0u;
   const uint32_t most = 4u * uint32_t(one ? kAttendOccupancy<C, true> : kAttendOccupancy<C, false>);
   const uint32_t waves = a.waves < most ? a.waves : most, bytes = attend_lds<C, QD>(waves);
-  // LDS past 64 KiB has to be asked for.
-  if (bytes > 65536u) {
+  // LDS past 64 KiB, 2 KiB of it static, has to be asked for.
+  if (bytes > 65536u - 2048u) {
     const hipError_t e = hipFuncSetAttribute(one ? reinterpret_cast<const void*>(scored_attend_kernel<C, QD, PD, true>)
                                                  : reinterpret_cast<const void*>(scored_attend_kernel<C, QD, PD, false>),
                                              hipFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
@@ -726,6 +726,18 @@ inline hipError_t launch_attend_cache4(const ScoredArgs& a, hipStream_t stream) 
   return launch_attend_cache<Cache4<G, 1>>(a, stream);
 }
 
+// Loads a unit's code object by one of its kernels.
+template <typename K>
+inline hipError_t preload_kernel(K* kernel) {
+  hipFuncAttributes attr;
+  return hipFuncGetAttributes(&attr, reinterpret_cast<const void*>(kernel));
+}
+hipError_t preload_attend4_d64();
+hipError_t preload_attend4_d128();
+hipError_t preload_attend4_d256();
+hipError_t preload_attend8_d64();
+hipError_t preload_attend8_d128();
+hipError_t preload_attend8_d256();
 hipError_t launch_attend4_d64(const ScoredArgs& a, hipStream_t stream);
 hipError_t launch_attend4_d128(const ScoredArgs& a, hipStream_t stream);
 hipError_t launch_attend4_d256(const ScoredArgs& a, hipStream_t stream);

@@ -19,4 +19,12 @@ hipError_t launch_scored_attend(const ScoredArgs& a, hipStream_t stream) {
   return hipGetLastError();
 }
 
+hipError_t preload_scored() {
+  hipError_t (*const units[])() = {preload_attend4_d64,  preload_attend4_d128,  preload_attend4_d256, preload_attend8_d64,
+                                   preload_attend8_d128, preload_attend8_d256, preload_scored_weights, preload_cache4, preload_evict};
+  for (const auto unit : units)
+    if (const hipError_t e = unit(); e != hipSuccess) return e;
+  return preload_kernel(scored_merge_kernel<64>);
+}
+
 }  // namespace kvb

@@ -3,4 +3,5 @@
 
 namespace kvb {
 hipError_t launch_attend4_d256(const ScoredArgs& a, hipStream_t stream) { return launch_attend_cache4<8>(a, stream); }
+hipError_t preload_attend4_d256() { return preload_kernel(scored_attend_kernel<Cache4<8, 1>, 2, 2, true>); }
 }  // namespace kvb

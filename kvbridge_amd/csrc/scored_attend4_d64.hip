@@ -3,4 +3,5 @@
 
 namespace kvb {
 hipError_t launch_attend4_d64(const ScoredArgs& a, hipStream_t stream) { return launch_attend_cache4<2>(a, stream); }
+hipError_t preload_attend4_d64() { return preload_kernel(scored_attend_kernel<Cache4<2, 1>, 2, 2, true>); }
 }  // namespace kvb

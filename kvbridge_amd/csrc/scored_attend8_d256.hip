@@ -5,4 +5,5 @@ namespace kvb {
 hipError_t launch_attend8_d256(const ScoredArgs& a, hipStream_t stream) {
   return launch_attend_cache<Cache8<8>>(a, stream);
 }
+hipError_t preload_attend8_d256() { return preload_kernel(scored_attend_kernel<Cache8<8>, 2, 2, true>); }
 }  // namespace kvb

@@ -8,7 +8,7 @@
 namespace kvb {
 namespace {
 
-// Threads of a grid dimension are counted in 32 bits, and work-groups have 256.
+// Threads of a grid dimension are counted in 32 bits; work-groups of 256 threads.
 constexpr uint64_t kMaxGroups = (uint64_t(1) << 24) - 1;
 
 const char* cache_error(uint32_t kv_heads, uint32_t dim, uint32_t page_tokens, uint32_t pages, uint32_t kv_bits) {
@@ -121,7 +121,7 @@ const char* scored_error(const kvb_scored_shape& s) {
     return "batch row/head product exceeds the grid limit";
   const ScoredSplits p = scored_splits(s);
   if (p.splits > 65535) return "split count exceeds 65535";
-  if (uint64_t(s.kv_heads) * scored_blocks(s) * p.items > kMaxGroups)
+  if (uint64_t(s.kv_heads) * scored_blocks(s) * p.items * 64 * p.waves > 0xffffffffull)
     return "split and head product exceeds the grid limit";
   return nullptr;
 }

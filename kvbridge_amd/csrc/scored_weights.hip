@@ -50,8 +50,8 @@ struct WeightBlock {
   float m[16], per_l[16], slope[16];
   int back[16];
 };
-template <class C, int QD>
-constexpr uint32_t kBlocksAtOnce = 65536u / sizeof(WeightBlock<C, QD>);
+template <class C, int QD>  // 64 KiB less the static LDS
+constexpr uint32_t kBlocksAtOnce = (65536u - 256u) / sizeof(WeightBlock<C, QD>);
 
 template <class C, int QD, bool ONE>
 __global__ __launch_bounds__((256 * kWeightOccupancy<C>), (kWeightOccupancy<C>)) void scored_weights_kernel(const ScoredArgs a) {
@@ -270,6 +270,11 @@ hipError_t launch_scored_weights(const ScoredArgs& a, hipStream_t stream) {
   if (a.dim == 64u) return launch_cache<Cache8<2>>(a, stream);
   if (a.dim == 128u) return launch_cache<Cache8<4>>(a, stream);
   return launch_cache<Cache8<8>>(a, stream);
+}
+
+hipError_t preload_scored_weights() {
+  hipFuncAttributes attr;
+  return hipFuncGetAttributes(&attr, reinterpret_cast<const void*>(&scored_weights_kernel<Cache4<2, 1>, 2, true>));
 }
 
 }  // namespace kvb

@@ -1,0 +1,197 @@
+"""Calls on a 4- or 8-bit cache at their ends, on the GPU against the plain
+64-bit forms: many head-rows, every column layout over long contexts, one
+sequence over more items than a merge holds at once, hundreds of sequences,
+graphs captured before any eager call, two streams at a time, and selections
+over more tokens than a work-group holds."""
+import numpy as np
+import pytest
+
+import kvbridge_amd as kvb
+
+from cache_forms import Attend, Case, check_attention
+from test_gpu_evict import Evict, select_plain, weights_of
+from test_gpu_scored import expected_weights
+
+pytestmark = pytest.mark.gpu
+
+
+def check_weights(case, t, call, fresh):
+    """Tolerance: score and m off by delta each and l by 2 delta (check_attention),
+    fewer than 2^5 fp32 roundings of sums of positive terms."""
+    import torch
+
+    kvb.accumulate_weights(call.s, call.inp, call.m, call.l, t["weights"], fresh)
+    torch.cuda.synchronize()
+    want = expected_weights(case, case.weights, fresh)
+    _, _, _, bounds, _ = case.attention()
+    delta = 32 * 2.0 ** -24 * bounds.max() + 8 * 2.0 ** -24 * case.cap + 2.0 ** -22
+    got = t["weights"].cpu().numpy()
+    assert np.all(np.abs(got - want) <= (4 * delta + 2.0 ** -18) * np.abs(want) + 2.0 ** -30), np.abs(got - want).max()
+
+
+MANY = [
+    # bits, rows, q_heads, kv_heads, dim, page, kind: the weights' Q operands take more than one pass at the last sizes
+    (4, 9, 8, 1, 256, 16, "f32"),
+    (4, 16, 16, 2, 128, 32, "bf16"),
+    (4, 30, 8, 1, 64, 8, "f32"),
+    (8, 9, 8, 1, 256, 32, "f32"),
+    (8, 16, 16, 2, 128, 24, "f16"),
+    (8, 70, 4, 1, 64, 16, "f32"),
+]
+
+
+@pytest.mark.parametrize("case", MANY)
+@pytest.mark.parametrize("forms", [{}, {"window": 40, "prefix": 3}])
+def test_many_head_rows(gpu, case, forms):
+    bits, rows, qh, kvh, dim, page, kind = case
+    c = Case(bits, [75, 300, 0, 131], rows, qh, kvh, dim, page, seed=31, kind=kind, **forms)
+    c.qpos[2] = -1
+    t = c.to_device()
+    want = c.attention()
+    for fused in (True, False):
+        call = Attend(c, t, "f32", fused)()
+        check_attention(c, call.read(), "f32", want)
+    check_weights(c, t, call, 7)
+
+
+COLUMNS = [
+    # bits, q_heads, kv_heads, dim: head-rows over 8, 4, 2 and 1 columns each
+    (4, 4, 2, 256), (4, 8, 2, 256), (4, 16, 2, 256),
+    (4, 4, 4, 128), (4, 16, 2, 128), (4, 32, 2, 128),
+    (4, 16, 2, 64), (4, 32, 2, 64),
+    (8, 8, 2, 64), (8, 8, 2, 128), (8, 8, 2, 256),
+]
+
+
+@pytest.mark.parametrize("case", COLUMNS)
+@pytest.mark.parametrize("page", [16, 64])
+def test_shared_out_items(gpu, case, page):
+    """Items by length (no split size named): one long sequence beside short ones."""
+    bits, qh, kvh, dim = case
+    c = Case(bits, [4001, 20, 9000, 641], 1, qh, kvh, dim, page, seed=32, kind="f16")
+    t = c.to_device()
+    want = c.attention()
+    for fused in (True, False):
+        call = Attend(c, t, "f32", fused)
+        check_attention(c, call().read(), "f32", want)
+        first = [x.clone() for x in (call.m, call.l, call.out)]
+        call().read()  # the same workspaces: the same bits
+        assert all(bool((a == b).all()) for a, b in zip(first, (call.m, call.l, call.out)))
+    check_weights(c, t, call, 0)
+
+
+@pytest.mark.parametrize("qh,kvh,dim,tokens", [(2, 2, 64, 33000), (8, 1, 128, 70000)])
+def test_one_sequence_over_more_items_than_a_merge_takes_at_once(gpu, qh, kvh, dim, tokens):
+    c = Case(4, [tokens], 1, qh, kvh, dim, 64, seed=33, kind="f16")
+    t = c.to_device()
+    want = c.attention()
+    for fused in (True, False):
+        call = Attend(c, t, "f32", fused)
+        assert kvb.scored_item_count(call.s) > 64
+        check_attention(c, call().read(), "f32", want)
+    check_weights(c, t, call, 0)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("batch", [70, 256, 300])
+def test_hundreds_of_sequences(gpu, bits, batch):
+    """Up to 256 sequences share the items out, above them every one gets the same number."""
+    lengths = np.random.default_rng(batch).integers(0, 150, batch)
+    lengths[batch // 2] = 1500
+    c = Case(bits, lengths, 1, 4, 2, 64, 16, seed=34, kind="bf16", window=100)
+    t = c.to_device()
+    want = c.attention()
+    for fused in (True, False):
+        call = Attend(c, t, "f32", fused)()
+        check_attention(c, call.read(), "f32", want)
+    check_weights(c, t, call, 1)
+
+
+@pytest.mark.parametrize("bits,qh,kvh,dim", [(4, 32, 2, 128), (8, 16, 2, 256), (4, 4, 2, 128), (4, 32, 2, 256)])
+def test_capture_without_an_eager_call(gpu, bits, qh, kvh, dim):
+    """After preloading, the first call of a shape may be a captured one, also
+    where a work-group needs more than 64 KiB of LDS."""
+    import torch
+
+    assert kvb.preload_attention_kernels() == 0
+    c = Case(bits, [3000], 1, qh, kvh, dim, 64, seed=35, kind="f32")
+    t = c.to_device()
+    calls = [Attend(c, t, "f32", fused) for fused in (True, False)]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for call in calls:
+            call()
+    want = c.attention()
+    for _ in range(3):
+        for call in calls:
+            call.out.fill_(float("nan"))
+        graph.replay()
+        for call in calls:
+            check_attention(c, call.read(), "f32", want)
+
+
+def test_two_streams_at_a_time(gpu):
+    """Calls on two streams with workspaces of their own, and captured graphs of
+    each replayed beside each other, give the bits of calls alone."""
+    import torch
+
+    cases = [Case(4, [2000, 900], 1, 8, 2, 128, 32, seed=36, kind="f16"), Case(8, [1700, 1200], 2, 8, 2, 64, 16, seed=37)]
+    ts = [c.to_device() for c in cases]
+    calls = [Attend(c, t, "f32")() for c, t in zip(cases, ts)]
+    alone = [call.read() for call in calls]
+    for c, got in zip(cases, alone):
+        check_attention(c, got, "f32")
+    streams = [torch.cuda.Stream() for _ in calls]
+    for _ in range(5):
+        for call, s in zip(calls, streams):
+            s.wait_stream(torch.cuda.current_stream())
+            call(s)
+            call(s)
+    for call, want in zip(calls, alone):
+        assert all(np.array_equal(a, b) for a, b in zip(call.read(), want))
+    graphs = []
+    for call in calls:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            call()
+        graphs.append(g)
+    for _ in range(5):
+        for g, s in zip(graphs, streams):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for call, want in zip(calls, alone):
+            assert all(np.array_equal(a, b) for a, b in zip(call.read(), want))
+
+
+@pytest.mark.parametrize("lengths,keep,how", [([70001, 32769, 32768], 5000, "random"), ([66000], 33000, "equal"),
+                                              ([40000, 100], 39999, "few")])
+def test_select_over_more_tokens_than_a_work_group_holds(gpu, lengths, keep, how):
+    import torch
+
+    c = Case(4, lengths, 1, 1, 1, 64, 64, seed=38, spare=1)
+    c.weights = weights_of(c, how, np.random.default_rng(39))
+    e = Evict(c, c.to_device(), keep, 3, 17)
+    e.select()
+    torch.cuda.synchronize()
+    got = e.kept.cpu().numpy()
+    for b, ids in enumerate(select_plain(c, c.weights, keep, 3, 17)):
+        assert got[b, :len(ids)].tolist() == ids, b
+
+
+def test_one_token_kept_of_one(gpu):
+    """The smallest eviction: every sequence one token, kept and moved."""
+    import torch
+
+    c = Case(8, [1, 1], 1, 1, 1, 64, 8, seed=40, spare=2)
+    t = c.to_device()
+    e = Evict(c, t, 1, 0, 0)
+    e.select()
+    e.move()
+    torch.cuda.synchronize()
+    assert e.kept.tolist() == [[0], [0]] and e.starts.tolist() == [0, 1, 2]
+    for b in range(2):
+        src, dst = int(c.table[b]), int(c.free[b])
+        assert torch.equal(t["k"][src][:, 0], t["k"][dst][:, 0]) and torch.equal(t["v"][src][..., 0], t["v"][dst][..., 0])
