@@ -71,7 +71,7 @@ struct AttendState {
   f32x4 acc[2 * C::kGroups];
   float mid[C::kBits == 4 ? C::kH : 1];
   float mtop, l;         // maximum of the lane's scores, sum
-  float ref, down, vf;   // reference, ve - reference, 2^ve
+  float ref, down, vf;   // reference, ve - reference, 2^ve (F = 1: the largest of the row's)
   int ve;
 };
 constexpr float kNoRef = -0x1p100f;  // below any score's exponent
@@ -87,6 +87,13 @@ struct ToTop {
 __device__ __forceinline__ ToTop to_top(float ref, int ve, float top) {
   const float t2 = top * kLog2e, up = __builtin_ceilf(t2);
   return ToTop{__builtin_amdgcn_exp2f((up - t2) - fmaf(top, kLog2e, -t2)), int(fmaxf(ref - up, -1000.f)) - ve};
+}
+
+__device__ __forceinline__ float row_max_f16(float x) {
+  x = fmaxf(x, row_ror<8>(x));
+  x = fmaxf(x, row_ror<4>(x));
+  x = fmaxf(x, row_ror<2>(x));
+  return fmaxf(x, row_ror<1>(x));
 }
 
 // Moves the reference to the head-row's maximum and sets ve by the tile's
@@ -123,7 +130,9 @@ __device__ __forceinline__ void rescale(AttendState<C>& s, const float (&x)[8], 
   }
   s.ref = ref;
   s.ve = ve;
+  // One column per head-row: a lane holds parameters that all 16 of its row use.
   s.vf = ldexpf(1.f, ve);
+  if constexpr (C::kF == 1) s.vf = row_max_f16(s.vf);
   s.down = float(ve) - ref;
 }
 

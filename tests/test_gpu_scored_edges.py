@@ -8,7 +8,7 @@ import pytest
 
 import kvbridge_amd as kvb
 
-from cache_forms import Attend, Case, check_attention
+from cache_forms import Attend, Case, check_attention, encode4
 from test_gpu_evict import Evict, select_plain, weights_of
 from test_gpu_scored import expected_weights
 
@@ -195,3 +195,45 @@ def test_one_token_kept_of_one(gpu):
     for b in range(2):
         src, dst = int(c.table[b]), int(c.free[b])
         assert torch.equal(t["k"][src][:, 0], t["k"][dst][:, 0]) and torch.equal(t["v"][src][..., 0], t["v"][dst][..., 0])
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dim,heads", [(64, 16), (128, 16), (128, 8), (256, 16), (256, 4)])
+@pytest.mark.parametrize("at", [0, 12, 28])
+def test_head_rows_of_different_value_scales(gpu, bits, dim, heads, at):
+    """Head-rows of a block that meet their largest weights at values 2^14 apart,
+    then large values in four tokens of a tile: head h looks at dim h of K only.
+    Going backwards, head 0's best token of every tile holds tiny values, the
+    other heads weigh all tokens alike; in the first half the tokens from `at` on
+    have values of 1 and scores for head 0 that are 5 higher, the rest tiny ones."""
+    T = 2048
+    c = Case(bits, [T], 1, heads, 1, dim, 32, seed=41, kind="f32", scale=1.0)
+    rng = np.random.default_rng(42)
+    c.q[:] = 0
+    for h in range(heads):
+        c.q[0, h * dim + h] = 1.0
+    k, v = np.zeros((T, dim), np.float32), rng.standard_normal((T, dim)).astype(np.float32)
+    k[:, 0], k[:, heads:] = -30.0, 0.01
+    best = np.arange(T // 2, T, 32) + rng.integers(0, 32, T // 64)
+    k[best, 0] = 0.0
+    v[best] *= 2.0 ** -14
+    large = np.arange(0, T // 2).reshape(-1, 32)[:, at:at + 4].ravel()
+    k[large, 0] = 5.0
+    v[np.setdiff1d(np.arange(T // 2), large)] *= 2.0 ** -14
+    for i in range(T):
+        pg, sl = int(c.table[i // 32]), i % 32
+        for rows, codes, scales in ((k, c.k, c.ks), (v, c.v, c.vs)):
+            if bits == 4:
+                codes[pg, 0, sl], scales[pg, 0, sl] = encode4(rows[i])
+            else:
+                s = np.abs(rows[i]).max() / np.float32(127)
+                x = np.clip(np.rint(rows[i] / s), -127, 127).astype(np.int8)
+                scales[pg, 0, sl] = s
+                if codes is c.v:
+                    codes[pg, 0, :, sl] = x
+                else:
+                    codes[pg, 0, sl] = x
+    t = c.to_device()
+    for split in (0, T):
+        c.split_tokens = split
+        check_attention(c, Attend(c, t, "f32")().read(), "f32")
