@@ -723,13 +723,14 @@ inline hipError_t launch_attend_cache(const ScoredArgs& a, hipStream_t stream) {
   if (a.out_type == 3u) return launch_attend_kernel<C, QD, 1>(a, stream);
   return launch_attend_kernel<C, QD, 2>(a, stream);
 }
-// As many columns per head-row as there is room for, up to one per block (two
-// blocks per column at the least F > 1: with more the parameters take too many
-// registers).
+// A column per block where the head-rows leave room for that; at dim 256 else
+// two blocks per column (16 heads over 4, 4 x 32K: 47 us against 53 with one
+// column per head-row).  At dim 128 that takes 216 VGPRs, two waves per SIMD, and
+// one column per head-row is faster (64 heads over 8, 4 x 128K: 187 -> 165 us).
 template <int G>
 inline hipError_t launch_attend_cache4(const ScoredArgs& a, hipStream_t stream) {
   if (a.head_rows <= 16u / G) return launch_attend_cache<Cache4<G, G>>(a, stream);
-  if constexpr (G > 2) {
+  if constexpr (G == 8) {
     if (a.head_rows <= 32u / G) return launch_attend_cache<Cache4<G, G / 2>>(a, stream);
   }
   return launch_attend_cache<Cache4<G, 1>>(a, stream);

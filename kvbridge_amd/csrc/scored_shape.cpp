@@ -50,10 +50,10 @@ constexpr uint64_t kCus = 256;
 
 // Waves of the attention kernel that a CU holds (kAttendOccupancy in
 // scored_attend.h).  One more wave per SIMD with spills inside the tile loop cost
-// a third to a half (16 ragged sequences 78 -> 160 us, 4 x 128K 186 -> 266).
+// a third to a half (16 ragged sequences 78 -> 160 us, four of 128K 186 -> 266).
 uint32_t resident_waves(const kvb_scored_shape& s) {
   const uint64_t head_rows = uint64_t(s.rows) * (s.q_heads / s.kv_heads), blocks = s.dim / 32;
-  const bool half = s.kv_bits == 4 && s.dim > 64 && head_rows > 16 / blocks && head_rows <= 32 / blocks;
+  const bool half = s.kv_bits == 4 && s.dim > 128 && head_rows > 16 / blocks && head_rows <= 32 / blocks;
   return s.dim == 256 || half || (s.kv_bits == 8 && s.page_tokens % 32 != 0) ? 8 : 12;
 }
 
@@ -96,9 +96,9 @@ ScoredSplits scored_splits(const kvb_scored_shape& s) {
 // One work-group's merge reads the partials of its head-rows past its L2, a
 // second launch spreads that over a work-group per head-row.  Measured (us, one
 // launch against two) by the sets of four dims that a thread of the first has to
-// add: 1 (int8, window, 32 sequences) 111 / 114, 3 (16 ragged ones) 78.7 / 79.6,
-// 4 (four of 128K) 184 / 181, 5 (one of 64K) 27.7 / 24.8, 21 (24 heads of 256 over
-// 8 rows) 38.1 / 34.2.
+// add: 1 (int8, window, 32 sequences) 111 / 114, 3 (16 ragged ones) 78.7 / 79.6, 3
+// (four of 128K, 64 heads) 115.5 / 115.3, 5 (one of 64K) 27.7 / 24.8, 21 (24 heads
+// of 256 over 8 rows) 38.1 / 34.2.
 bool scored_one_launch(const kvb_scored_shape& s, const ScoredSplits& p) {
   const uint64_t head_rows = std::min<uint64_t>(16, uint64_t(s.rows) * (s.q_heads / s.kv_heads));
   return p.items / s.batch * head_rows * (s.dim / 4) <= 3 * 64 * p.waves;

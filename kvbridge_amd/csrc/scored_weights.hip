@@ -253,7 +253,7 @@ hipError_t launch_cache(const ScoredArgs& a, hipStream_t stream) {
 template <int G>
 hipError_t launch_cache4(const ScoredArgs& a, hipStream_t stream) {  // as launch_attend_cache4
   if (a.head_rows <= 16u / G) return launch_cache<Cache4<G, G>>(a, stream);
-  if constexpr (G > 2) {
+  if constexpr (G == 8) {
     if (a.head_rows <= 32u / G) return launch_cache<Cache4<G, G / 2>>(a, stream);
   }
   return launch_cache<Cache4<G, 1>>(a, stream);
