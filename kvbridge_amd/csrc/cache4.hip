@@ -7,6 +7,10 @@
 // bytes, and a block's least and largest value are two DPP steps over the four
 // lanes.  Arithmetic is IEEE fp32 step by step, so the stored bits are those of
 // any correctly rounded evaluation of the same formula.
+// Measured at 16,384 tokens of 8 kv heads, dim 128: writing fp16 rows 28-33 us
+// (88 MB, 2.7-3.1 TB/s; with a division per element 37), reading them back as
+// fp32 26 us (155 MB, 5.9 TB/s); 64 tokens 4.4 and 2.9 us, launch and one chain
+// of loads.
 #include <cfloat>
 
 #include "device_common.h"

@@ -9,6 +9,10 @@
 // tokens in order: above the key they stay, of those equal to it the first ones.
 // Move: one work-group per 64 kept tokens and kv head copies rows in 16-byte
 // pieces (int8 V, dim-major, byte by byte gathered to dwords).
+// Measured at 16 sequences of up to 32K tokens cut to 4,096, 8 kv heads of dim
+// 128, 4 bits: keys 8.5 us, pick 22.5 (a work-group per sequence: LDS atomics and
+// barriers), move 50-69 (168 MB of rows; kept rows of 64 bytes share the memory's
+// 128-byte lines with others).
 #include "device_common.h"
 #include "scored.h"
 

@@ -31,9 +31,9 @@
 // applies the parameters of its H blocks only (loaded by itself), and a sum over
 // F neighbouring lanes makes the score; likewise the weights times the steps
 // and the values at code 8.  That was 592 -> 350 vector instructions per tile
-// at dim 128 and four head-rows (F = 4).  F = 1 (more head-rows than 16 / F):
-// the parameters of a lane's tokens lie in the 16 lanes of its row and are read
-// by DPP row broadcasts.
+// at dim 128 and four head-rows (F = 4).  F = 1 (more head-rows): the parameters
+// of a lane's tokens lie in the 16 lanes of its row and are read by DPP row
+// broadcasts inside the multiply-adds.
 // 8 bits: codes are converted exactly (i8x8_to_f16), the per-token scale
 // multiplies the sum.
 //
@@ -57,8 +57,8 @@ typedef uint32_t u32x4_s __attribute__((ext_vector_type(4)));
 
 constexpr uint32_t kTileTokens = 32;
 
-// Lane J of each 16-lane row.  Every
-// lane must be active where it is called: outside of selects and branches.
+// Lane J of each 16-lane row.  Every lane must be active where it is called:
+// outside of selects and branches.
 template <int J>
 __device__ __forceinline__ float bc(float x) {
   return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x150 + J, 0xF, 0xF, true));
@@ -839,10 +839,10 @@ __device__ __forceinline__ int near(int64_t d) {
 }
 
 // Score forms on a tile's products: factor, cap, bias by distance, and -inf
-// where the tile is masked and the token not visible.  Scores stay in natural units: their difference
-// to a reference is taken first and then multiplied by log2(e) for the
-// exponential.  With the two constants in one rounded factor instead, l of 512
-// tokens was off by 1.1e-6, since every score carried the same relative error.
+// where the tile is masked and the token not visible.  Scores stay in natural
+// units and are multiplied by log2(e) inside the exponent's fma: with scale and
+// log2(e) in one rounded factor l of 512 tokens was off by 1.1e-6, since every
+// score carried the same relative error.
 struct ScoreForm {
   float factor, cap, inv_cap, slope;
   int back;  // this row's position less the first row's

@@ -5,19 +5,26 @@
 // waves the split's 32-token tiles in turn.  It has all the waves that a CU
 // holds of this kernel (12 or 8: few partials, which it can merge itself) where
 // the sequences are few, and 4 where they are many and finer parts balance
-// better: 16 ragged sequences 78 us against 85, one of 64K tokens 27.7 against
-// 27.0 (scored_splits in scored_shape.cpp).  One pass over the
-// tokens with a running reference mref per head-row (not the maximum itself:
-// it moves only when a score exceeds it by 5.5, so that most tiles rescale
-// nothing), l in fp32, and the output's numerators in MFMA
-// accumulators whose column is the head-row, so a rescale is lane-local.
+// better (16 ragged sequences 78 us against 85; split_items in
+// scored_shape.cpp).  One pass over the tokens with a running reference per
+// head-row (not the maximum itself: it moves only when a score exceeds it by
+// 5.5, so that most tiles rescale nothing), l in fp32, and the output's
+// numerators in MFMA accumulators whose column is the head-row, so a rescale is
+// lane-local.
 //
 // PV: the weight of token t for the dims of block g is p_t * step_{t,g}; times
 // 2^ve it enters the product as one fp16 (PD 1: bf16 output, whose step is
 // eight times coarser) or as two (PD 2).  ve is set per head-row where its
-// weights are largest, and again when mref moves or when a step grows by 2^8,
-// which keeps fp16 from overflowing for any steps.  The blocks' values at code
-// 8 add sum_t p_t mid_{t,g} in fp32.
+// weights are largest, and again when the reference moves or when a step times
+// the largest 2^ve beside it passes 2^7, which keeps fp16 from overflowing for
+// any steps.  The blocks' values at code 8 add sum_t p_t mid_{t,g} in fp32.
+//
+// What bounds it: long contexts the cache's bytes (16 ragged sequences of up to
+// 32K tokens, 32 heads over 8 of dim 128: 77.5 us, 4.3 TB/s; four of 128K, 64
+// heads: 165 us, 4.1 TB/s; int8, 32 windows of 4,096, dim 256: 109.7 us, 4.6
+// TB/s), short ones the chain of dependent loads from the item to its pages, K
+// and the merge (512 tokens: 10 us), many head-rows of dim 256 the arithmetic of
+// a tile, 4 us of a wave with two on a SIMD (48 head-rows, 8K tokens: 34 us).
 #pragma once
 #include "scored.h"
 

