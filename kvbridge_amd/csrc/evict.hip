@@ -4,15 +4,17 @@
 // uint32 of its weight (the kv heads summed in fp64, rounded to fp32; always-
 // kept tokens the largest key, NaN the least).  evict_pick_kernel, one
 // work-group per sequence, finds the key of rank n by three radix passes of 11,
-// 11 and 10 bits over LDS histograms (four copies: most keys share few leading
-// digits), the keys of up to 32K tokens staying in registers, then writes the
-// tokens in order: above the key they stay, of those equal to it the first ones.
+// 11 and 10 bits over LDS histograms, the keys of up to 32K tokens staying in
+// registers, then writes the tokens in order: above the key they stay, of those
+// equal to it the first ones.
 // Move: one work-group per 64 kept tokens and kv head copies rows in 16-byte
 // pieces (int8 V, dim-major, byte by byte gathered to dwords).
 // Measured at 16 sequences of up to 32K tokens cut to 4,096, 8 kv heads of dim
-// 128, 4 bits: keys 8.5 us, pick 22.5 (a work-group per sequence: LDS atomics and
-// barriers), move 50-69 (168 MB of rows; kept rows of 64 bytes share the memory's
-// 128-byte lines with others).
+// 128, 4 bits: keys 6.0 us (8.5 with a token per thread), pick 19.5 (a work-group
+// per sequence; 22.5 with bounds checked at every key and six barriers a pass
+// instead of three), move 50-70 (168 MB of rows; kept rows of 64 bytes share the
+// memory's 128-byte lines with others: four heads to a work-group changed
+// nothing).  Two sequences of 2K: 2.3, 8.2 and 6.8.
 #include "device_common.h"
 #include "scored.h"
 
@@ -21,60 +23,100 @@ namespace {
 
 typedef uint32_t u32x4_e __attribute__((ext_vector_type(4)));
 
-constexpr uint32_t kPickThreads = 1024, kPickWaves = kPickThreads / 64, kBins = 2048, kCopies = 4;
+constexpr uint32_t kPickThreads = 1024, kPickWaves = kPickThreads / 64, kBins = 2048;
 
 __device__ __forceinline__ ScoredSeq evict_seq(const EvictArgs& a, uint32_t b) {
   return clamp_seq(a.seq_starts[b], a.seq_starts[b + 1u], a.page_offsets[b], a.total_tokens, a.table_entries, a.page_tokens,
                    a.max_tokens);
 }
 
+// Four tokens a thread, which share a page (page_tokens is a multiple of 8).
+template <bool VEC>
 __global__ __launch_bounds__(256) void evict_keys_kernel(const EvictArgs a) {
-  const uint32_t b = blockIdx.y, t = blockIdx.x * 256u + threadIdx.x;
+  const uint32_t b = blockIdx.y, t = (blockIdx.x * 256u + threadIdx.x) * 4u;
   const ScoredSeq e = evict_seq(a, b);
   if (t >= e.tokens || e.tokens <= a.keep) return;  // all stay: no key is looked at
-  uint32_t key = 0xffffffffu;
-  if (t >= a.sink && e.tokens - t > a.recent) {
-    const uint32_t lp = t / a.page_tokens, slot = t - lp * a.page_tokens;
-    uint32_t page = a.page_table[e.table_off + lp];
-    page = page < a.pages ? page : a.pages - 1u;
-    const float* w = a.weights_in + uint64_t(page) * a.kv_heads * a.page_tokens + slot;
-    double sum = 0.0;
-    for (uint32_t h0 = 0; h0 < a.kv_heads; h0 += 8u) {  // eight heads' loads at once
-      float x[8];
+  const uint32_t lp = t / a.page_tokens, slot = t - lp * a.page_tokens;
+  uint32_t page = a.page_table[e.table_off + lp];
+  page = page < a.pages ? page : a.pages - 1u;
+  const float* w = a.weights_in + uint64_t(page) * a.kv_heads * a.page_tokens + slot;
+  double sum[4] = {0.0, 0.0, 0.0, 0.0};
+  for (uint32_t h0 = 0; h0 < a.kv_heads; h0 += 8u) {  // eight heads' loads at once
+    f32x4 x[8];
 #pragma unroll
-      for (uint32_t i = 0; i < 8u; ++i) x[i] = h0 + i < a.kv_heads ? w[uint64_t(h0 + i) * a.page_tokens] : 0.f;
-#pragma unroll
-      for (uint32_t i = 0; i < 8u; ++i) sum += h0 + i < a.kv_heads ? double(x[i]) : 0.0;
+    for (uint32_t i = 0; i < 8u; ++i) {
+      const float* p = w + uint64_t(h0 + i) * a.page_tokens;
+      x[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (h0 + i >= a.kv_heads) continue;
+      if constexpr (VEC) x[i] = *reinterpret_cast<const f32x4*>(p);
+      else x[i] = f32x4{p[0], p[1], p[2], p[3]};
     }
-    const float f = float(sum) + 0.f;  // -0 becomes 0
-    const uint32_t u = __float_as_uint(f);
-    key = f != f ? 0u : ((u >> 31) != 0u ? ~u : u | 0x80000000u);
+#pragma unroll
+    for (uint32_t i = 0; i < 8u; ++i)
+#pragma unroll
+      for (uint32_t c = 0; c < 4u; ++c) sum[c] += double(x[i][c]);
   }
-  a.scratch[uint64_t(b) * a.scratch_stride + t] = key;
+  u32x4_e keys;
+#pragma unroll
+  for (uint32_t c = 0; c < 4u; ++c) {
+    const float f = float(sum[c]) + 0.f;  // -0 becomes 0
+    const uint32_t u = __float_as_uint(f), key = f != f ? 0u : ((u >> 31) != 0u ? ~u : u | 0x80000000u);
+    keys[c] = t + c >= a.sink && t + c + a.recent < e.tokens ? key : 0xffffffffu;
+  }
+  *reinterpret_cast<u32x4_e*>(a.scratch + uint64_t(b) * a.scratch_stride + t) = keys;
 }
 
-// A thread's keys of a chunk of up to 32K tokens: every wave has 256 * rounds
-// consecutive ones (rounds: as few as cover the sequence), in the order (i, lane, c).
+// A thread's keys of a chunk of up to 32K tokens: 4 * rounds consecutive ones
+// (rounds: as few as cover the sequence).
 constexpr uint32_t kLaneKeys = 8, kChunkKeys = kPickThreads * 4 * kLaneKeys;
 struct LaneKeys {
   u32x4_e k[kLaneKeys];
-  uint32_t rounds, first;  // first: the wave's first token
-  __device__ __forceinline__ uint32_t token(uint32_t i, uint32_t c) const { return first + i * 256u + (threadIdx.x & 63u) * 4u + c; }
-  // All loads at once.  Past the last token the scratch holds anything.
+  uint32_t rounds, first;  // first: the thread's first token
+  __device__ __forceinline__ uint32_t token(uint32_t i, uint32_t c) const { return first + i * 4u + c; }
+  // All loads at once.  Past the last token, where the scratch holds anything, the
+  // least key: it comes after every token of the same key and is never reached.
   __device__ __forceinline__ void load(const uint32_t* keys, uint32_t chunk, uint32_t tokens, uint32_t stride) {
     rounds = tokens >= kChunkKeys ? kLaneKeys : (tokens + kPickThreads * 4u - 1u) / (kPickThreads * 4u);
-    first = chunk * kChunkKeys + uint32_t(__builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6))) * (256u * rounds);
+    first = chunk * kChunkKeys + threadIdx.x * (4u * rounds);
 #pragma unroll
     for (uint32_t i = 0; i < kLaneKeys; ++i) {
       const uint32_t t = token(i, 0u);
       k[i] = i < rounds && t < stride ? *reinterpret_cast<const u32x4_e*>(keys + t) : u32x4_e{0u, 0u, 0u, 0u};
     }
+    if (first + 4u * rounds > tokens) {
+#pragma unroll
+      for (uint32_t i = 0; i < kLaneKeys; ++i)
+#pragma unroll
+        for (uint32_t c = 0; c < 4u; ++c) k[i][c] = token(i, c) < tokens ? k[i][c] : 0u;
+    }
   }
 };
 
+// The keys' sums over the threads before this one, and over all.
+struct Before {
+  uint32_t mine, all;
+};
+__device__ __forceinline__ Before sum_before(uint32_t x, uint32_t (&waves)[kPickWaves]) {
+  const uint32_t upto = wave_scan(x), wave = threadIdx.x >> 6;
+  if ((threadIdx.x & 63u) == 63u) waves[wave] = upto;
+  __syncthreads();
+  Before r{upto - x, 0u};
+#pragma unroll
+  for (uint32_t w = 0; w < kPickWaves; ++w) {
+    const uint32_t n = waves[w];
+    r.mine += w < wave ? n : 0u;
+    r.all += n;
+  }
+  return r;
+}
+
 __global__ __launch_bounds__(kPickThreads) void evict_pick_kernel(const EvictArgs a) {
-  __shared__ uint32_t hist[kCopies][kBins];
-  __shared__ uint32_t found[2], wave_gt[kPickWaves], wave_eq[kPickWaves];
+  // The three passes' histograms beside each other, so that one barrier clears
+  // all of them.  Most keys share few leading digits: neighbouring lanes count in
+  // copies of their own, which begin in different banks.
+  constexpr uint32_t kBinsOf[3] = {kBins, kBins, 1024u}, kCopiesOf[3] = {4u, 2u, 2u}, kShift = 8u;
+  __shared__ uint32_t hist[4u * (kBins + kShift) + 2u * (kBins + kShift) + 2u * (1024u + kShift)];
+  __shared__ uint32_t found[3][2], waves[3][kPickWaves], wave_gt[kPickWaves], wave_eq[kPickWaves];
   const uint32_t b = blockIdx.x, tid = threadIdx.x, lane = tid & 63u;
   const uint32_t wave = uint32_t(__builtin_amdgcn_readfirstlane(int(tid >> 6)));
   const ScoredSeq e = evict_seq(a, b);
@@ -104,54 +146,51 @@ __global__ __launch_bounds__(kPickThreads) void evict_pick_kernel(const EvictArg
 
   // The n-th largest key: its digits from the top, `want` its rank among the
   // keys that share the digits found so far.
+  for (uint32_t i = tid; i < sizeof(hist) / 4u; i += kPickThreads) hist[i] = 0u;
+  __syncthreads();
   uint32_t prefix = 0, mask = 0, want = n;
+  uint32_t* bins = hist;
+#pragma unroll
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
-    const uint32_t digits = pass == 2 ? 1024u : kBins;
-    for (uint32_t i = tid; i < kCopies * kBins; i += kPickThreads) (&hist[0][0])[i] = 0u;
-    __syncthreads();
-    uint32_t* const h = hist[wave % kCopies];
+    const uint32_t digits = kBinsOf[pass], copies = kCopiesOf[pass], stride = digits + kShift;
+    uint32_t* const h = bins + lane % copies * stride;
     for (uint32_t chunk = 0; chunk < chunks; ++chunk) {
       if (chunks > 1u) own.load(keys, chunk, e.tokens, a.scratch_stride);
 #pragma unroll
       for (uint32_t i = 0; i < kLaneKeys; ++i) {
         if (i >= own.rounds) break;
+        if (own.token(i, 0u) >= e.tokens) continue;
 #pragma unroll
         for (uint32_t c = 0; c < 4u; ++c)
-          if (own.token(i, c) < e.tokens && (own.k[i][c] & mask) == prefix)
-            atomicAdd(&h[(own.k[i][c] >> shift) & (digits - 1u)], 1u);
+          if (pass == 0 || (own.k[i][c] & mask) == prefix) atomicAdd(&h[(own.k[i][c] >> shift) & (digits - 1u)], 1u);
       }
     }
     __syncthreads();
-    // Thread t has the bins top - 2 t and the next below (one bin in the last
-    // pass): keys in them, in the wave's bins up to them, in the waves before.
+    // Thread t has the bins top - 2 t and the next below (one bin in the last pass).
     const uint32_t per = digits / kPickThreads, bin = digits - 1u - tid * per;
     uint32_t c0 = 0, c1 = 0;
 #pragma unroll
-    for (uint32_t c = 0; c < kCopies; ++c) {
-      c0 += hist[c][bin];
-      c1 += per == 2u ? hist[c][bin - 1u] : 0u;
+    for (uint32_t c = 0; c < copies; ++c) {
+      c0 += bins[c * stride + bin];
+      c1 += per == 2u ? bins[c * stride + bin - 1u] : 0u;
     }
-    const uint32_t upto = wave_scan(c0 + c1);
-    if (lane == 63u) wave_gt[wave] = upto;
-    __syncthreads();
-    uint32_t before = upto - c0 - c1;
-    for (uint32_t w = 0; w < wave; ++w) before += wave_gt[w];
+    const uint32_t before = sum_before(c0 + c1, waves[pass]).mine;
     if (before < want && want <= before + c0 + c1) {
       const bool second = want > before + c0;
-      found[0] = second ? bin - 1u : bin;
-      found[1] = want - before - (second ? c0 : 0u);
+      found[pass][0] = second ? bin - 1u : bin;
+      found[pass][1] = want - before - (second ? c0 : 0u);
     }
     __syncthreads();
-    prefix |= found[0] << shift;
-    want = found[1];
+    prefix |= found[pass][0] << shift;
+    want = found[pass][1];
     mask |= (digits - 1u) << shift;
-    __syncthreads();
+    bins += copies * stride;
   }
 
-  // Chunk by chunk every wave counts its keys above the n-th and equal to it,
-  // then writes those that stay behind what the waves before it keep.
-  uint32_t at0 = 0, eq0 = 0;  // kept, and equal keys met, before the chunk
+  // Chunk by chunk: a thread's first place is the number of keys before its own
+  // that are above the n-th, and of those equal to it the first `want`.
+  uint32_t gt0 = 0, eq0 = 0;
   for (uint32_t chunk = 0; chunk < chunks; ++chunk) {
     if (chunks > 1u) own.load(keys, chunk, e.tokens, a.scratch_stride);
     uint32_t gt = 0, eq = 0;
@@ -159,56 +198,23 @@ __global__ __launch_bounds__(kPickThreads) void evict_pick_kernel(const EvictArg
     for (uint32_t i = 0; i < kLaneKeys; ++i)
 #pragma unroll
       for (uint32_t c = 0; c < 4u; ++c) {
-        const bool in = i < own.rounds && own.token(i, c) < e.tokens;
-        gt += in && own.k[i][c] > prefix ? 1u : 0u;
-        eq += in && own.k[i][c] == prefix ? 1u : 0u;
+        gt += own.k[i][c] > prefix ? 1u : 0u;
+        eq += own.k[i][c] == prefix ? 1u : 0u;
       }
-    const uint32_t all_gt = uint32_t(__builtin_amdgcn_readlane(int(wave_scan(gt)), 63));
-    const uint32_t all_eq = uint32_t(__builtin_amdgcn_readlane(int(wave_scan(eq)), 63));
-    if (lane == 0u) {
-      wave_gt[wave] = all_gt;
-      wave_eq[wave] = all_eq;
-    }
-    __syncthreads();
-    uint32_t at = at0, eqs = eq0;
-    for (uint32_t w = 0; w < kPickWaves; ++w) {
-      const uint32_t room = want > eq0 ? want - eq0 : 0u, take = wave_gt[w] + (wave_eq[w] < room ? wave_eq[w] : room);
-      if (w < wave) {
-        at += take;
-        eqs += wave_eq[w];
-      }
-      at0 += take;
-      eq0 += wave_eq[w];
-    }
-    __syncthreads();
+    if (chunk > 0u) __syncthreads();  // the last chunk's sums have been read
+    const Before g = sum_before(gt, wave_gt), q = sum_before(eq, wave_eq);
+    uint32_t rank = eq0 + q.mine, to = gt0 + g.mine + (rank < want ? rank : want);
+    gt0 += g.all;
+    eq0 += q.all;
 #pragma unroll
     for (uint32_t i = 0; i < kLaneKeys; ++i) {
       if (i >= own.rounds) break;
-      uint32_t lane_eq = 0;
-      bool is_eq[4], is_gt[4];
 #pragma unroll
       for (uint32_t c = 0; c < 4u; ++c) {
-        const bool in = i < own.rounds && own.token(i, c) < e.tokens;
-        is_gt[c] = in && own.k[i][c] > prefix;
-        is_eq[c] = in && own.k[i][c] == prefix;
-        lane_eq += is_eq[c] ? 1u : 0u;
+        const bool is_eq = own.k[i][c] == prefix;
+        if (own.k[i][c] > prefix || (is_eq && rank < want)) kept[to++] = own.token(i, c);
+        rank += is_eq ? 1u : 0u;
       }
-      const uint32_t eq_upto = wave_scan(lane_eq);
-      uint32_t rank = eqs + eq_upto - lane_eq, lane_stays = 0;
-      bool stays[4];
-#pragma unroll
-      for (uint32_t c = 0; c < 4u; ++c) {
-        stays[c] = is_gt[c] || (is_eq[c] && rank < want);
-        rank += is_eq[c] ? 1u : 0u;
-        lane_stays += stays[c] ? 1u : 0u;
-      }
-      const uint32_t upto = wave_scan(lane_stays);
-      uint32_t to = at + upto - lane_stays;
-#pragma unroll
-      for (uint32_t c = 0; c < 4u; ++c)
-        if (stays[c]) kept[to++] = own.token(i, c);
-      at += uint32_t(__builtin_amdgcn_readlane(int(upto), 63));
-      eqs += uint32_t(__builtin_amdgcn_readlane(int(eq_upto), 63));
     }
   }
 }
@@ -343,7 +349,9 @@ __global__ __launch_bounds__(256) void evict_move_kernel(const EvictArgs a) {
 }  // namespace
 
 hipError_t launch_evict_select(const EvictArgs& a, hipStream_t stream) {
-  evict_keys_kernel<<<dim3(a.max_tokens / 256u + (a.max_tokens % 256u != 0u ? 1u : 0u), a.batch), 256, 0, stream>>>(a);
+  const dim3 grid(a.max_tokens / 1024u + (a.max_tokens % 1024u != 0u ? 1u : 0u), a.batch);
+  if (reinterpret_cast<uintptr_t>(a.weights_in) % 16u == 0u) evict_keys_kernel<true><<<grid, 256, 0, stream>>>(a);
+  else evict_keys_kernel<false><<<grid, 256, 0, stream>>>(a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   evict_pick_kernel<<<a.batch, kPickThreads, 0, stream>>>(a);
@@ -367,7 +375,7 @@ hipError_t launch_evict_move(const EvictArgs& a, hipStream_t stream) {
 
 hipError_t preload_evict() {
   hipFuncAttributes attr;
-  return hipFuncGetAttributes(&attr, reinterpret_cast<const void*>(&evict_keys_kernel));
+  return hipFuncGetAttributes(&attr, reinterpret_cast<const void*>(&evict_keys_kernel<true>));
 }
 
 }  // namespace kvb

@@ -181,6 +181,24 @@ def test_select_over_more_tokens_than_a_work_group_holds(gpu, lengths, keep, how
         assert got[b, :len(ids)].tolist() == ids, b
 
 
+def test_select_from_weights_off_16_bytes(gpu):
+    """The weights are floats: no alignment beyond theirs is asked for."""
+    import torch
+
+    c = Case(4, [700, 33, 9], 1, 3, 3, 64, 24, seed=43, spare=1)
+    c.weights = weights_of(c, "odd", np.random.default_rng(44))
+    t = c.to_device()
+    e = Evict(c, t, 65, 1, 9)
+    want = select_plain(c, c.weights, 65, 1, 9)
+    room = torch.empty(t["weights"].numel() + 1, device=gpu)
+    off = room[1:].view(t["weights"].shape)
+    off.copy_(t["weights"])
+    kvb.evict_select(e.s, e.inp, off, e.scratch, e.kept, e.starts)
+    torch.cuda.synchronize()
+    got = e.kept.cpu().numpy()
+    assert [got[b, :len(w)].tolist() for b, w in enumerate(want)] == want
+
+
 def test_one_token_kept_of_one(gpu):
     """The smallest eviction: every sequence one token, kept and moved."""
     import torch
