@@ -7,10 +7,10 @@
 // bytes, and a block's least and largest value are two DPP steps over the four
 // lanes.  Arithmetic is IEEE fp32 step by step, so the stored bits are those of
 // any correctly rounded evaluation of the same formula.
-// Measured at 16,384 tokens of 8 kv heads, dim 128: writing fp16 rows 28-33 us
-// (88 MB, 2.7-3.1 TB/s; with a division per element 37), reading them back as
-// fp32 26 us (155 MB, 5.9 TB/s); 64 tokens 4.4 and 2.9 us, launch and one chain
-// of loads.
+// Measured at 16,384 tokens of 8 kv heads, dim 128: writing fp16 rows 26-31 us
+// (88 MB, 2.8-3.4 TB/s; the 672 vector instructions of a wave take 20 of them;
+// with a division per element 37), reading them back as fp32 26 us (155 MB, 5.9
+// TB/s); 64 tokens 4.4 and 2.9 us, launch and one chain of loads.
 #include <cfloat>
 
 #include "device_common.h"
@@ -36,16 +36,48 @@ __device__ __forceinline__ uint32_t bf16_bits(float x) {
 }
 __device__ __forceinline__ float from_bf16(uint32_t b) { return __uint_as_float(b << 16); }
 
-// clamp(rint(y / step), 0, 15) of the correctly rounded quotient, mostly without
-// the division: y * per, per the hardware reciprocal (1 ulp), is within 1.25 *
-// 2^-22 of it relatively, 2^-17 absolutely up to code 15 and a half, so where it
-// lies more than 2^-14 from a half the nearest integer is the same.  The rest
-// (one in 8,000, and any quotient that is not finite) divides.
-__device__ __forceinline__ uint32_t code_of(float y, float step, float per) {
-  const float q = y * per;
-  float c = __builtin_rintf(q);
-  if (!(fabsf(q - c) <= 0.5f - 0x1p-14f)) c = __builtin_rintf(y / step);
-  return uint32_t(fminf(fmaxf(c, 0.f), 15.f));
+// Eight codes clamp(rint(y / step), 0, 15), y = x - least, the quotient correctly
+// rounded, four bits each.  Mostly without the division: with the hardware
+// reciprocal (1 ulp) y * per is within 1.5 * 2^-23 of that quotient relatively,
+// 2^-18 absolutely up to code 15 and a half, so where it lies more than 2^-14
+// from a half the nearest integer is the same.  The rest (exact halves, one in
+// 700 of 16-bit sources, and any product that is not finite) divides.  Adding 1.5 *
+// 2^23 rounds to an integer in the low bits of the sum (quotients stay below
+// 2^20), so the codes are put together as the sums' bits, the constants' sum
+// taken off.
+__device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float least, float step) {
+  constexpr float kRound = 12582912.f;  // bits 0x4b400000
+  const float per = __builtin_amdgcn_rcpf(step);
+  uint32_t codes = 0u, constants = 0u;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float y = x[i] - least;
+    float r = fmaf(y, per, kRound);
+    if (!(fabsf(fmaf(y, per, -(r - kRound))) <= 0.5f - 0x1p-14f)) r = __builtin_rintf(y / step) + kRound;
+    codes += __float_as_uint(__builtin_amdgcn_fmed3f(r, kRound, kRound + 15.f)) << (4 * i);
+    constants += 0x4b400000u << (4 * i);
+  }
+  return codes - constants;
+}
+
+// The lane's 4 G bytes: byte i * G + g is byte i of block g's codes.
+template <int G>
+__device__ __forceinline__ void interleave(const uint32_t (&codes)[G], uint32_t (&packed)[G]) {
+  if constexpr (G == 2) {
+    packed[0] = __builtin_amdgcn_perm(codes[1], codes[0], 0x05010400u);
+    packed[1] = __builtin_amdgcn_perm(codes[1], codes[0], 0x07030602u);
+  } else {
+#pragma unroll
+    for (int h = 0; h < G / 4; ++h) {
+      const uint32_t* c = codes + 4 * h;
+      const uint32_t lo01 = __builtin_amdgcn_perm(c[1], c[0], 0x05010400u), hi01 = __builtin_amdgcn_perm(c[1], c[0], 0x07030602u);
+      const uint32_t lo23 = __builtin_amdgcn_perm(c[3], c[2], 0x05010400u), hi23 = __builtin_amdgcn_perm(c[3], c[2], 0x07030602u);
+      packed[h] = __builtin_amdgcn_perm(lo23, lo01, 0x05040100u);
+      packed[G / 4 + h] = __builtin_amdgcn_perm(lo23, lo01, 0x07060302u);
+      packed[2 * (G / 4) + h] = __builtin_amdgcn_perm(hi23, hi01, 0x05040100u);
+      packed[3 * (G / 4) + h] = __builtin_amdgcn_perm(hi23, hi01, 0x07060302u);
+    }
+  }
 }
 
 // Eight elements from p: 16-byte loads where the host has checked that every
@@ -86,20 +118,17 @@ __global__ __launch_bounds__(256) void append4_kernel(const Append4Args a) {
   float x[G][8];
 #pragma unroll
   for (int g = 0; g < G; ++g) load8<T, VEC>(src + 32 * g, x[g]);
-  uint32_t packed[G], word[G];
-#pragma unroll
-  for (int g = 0; g < G; ++g) packed[g] = 0u;
+  uint32_t codes[G], packed[G], word[G];
 #pragma unroll
   for (int g = 0; g < G; ++g) {
-    float lo = x[g][0], hi = x[g][0];
-    bool bad = !(fabsf(x[g][0]) <= FLT_MAX);
+    float lo = x[g][0], hi = x[g][0], odd = 0.f;
 #pragma unroll
-    for (int i = 1; i < 8; ++i) {
+    for (int i = 0; i < 8; ++i) {
       lo = fminf(lo, x[g][i]);
       hi = fmaxf(hi, x[g][i]);
-      bad = bad || !(fabsf(x[g][i]) <= FLT_MAX);
+      odd = fmaf(x[g][i], 0.f, odd);  // NaN once an element is not finite
     }
-    if (bad) hi = lo = __builtin_huge_valf();  // carried by hi to the other lanes
+    if (odd != 0.f) hi = lo = __builtin_huge_valf();  // carried by hi to the other lanes
     lo = fminf(lo, quad_xor<1>(lo));
     hi = fmaxf(hi, quad_xor<1>(hi));
     lo = fminf(lo, quad_xor<2>(lo));
@@ -109,23 +138,12 @@ __global__ __launch_bounds__(256) void append4_kernel(const Append4Args a) {
     uint32_t step_b = bf16_bits(fmaxf(hi - least, 0.f) / 15.f);
     const float step = from_bf16(step_b);
     const bool fine = hi <= FLT_MAX && fabsf(least) <= FLT_MAX && step <= FLT_MAX;
-    uint32_t codes = 0u;
-    if (fine && step > 0.f) {
-      const float per = __builtin_amdgcn_rcpf(step);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        codes |= code_of(x[g][i] - least, step, per) << (4 * i);
-      }
-    }
+    codes[g] = 0u;
+    if (fine && step > 0.f) codes[g] = codes_of(x[g], least, step);
     if (!fine) least_b = step_b = 0x7fc0u;
     word[g] = step_b << 16 | least_b;
-    // byte i of codes: dims 2 i, 2 i + 1 of the lane; its place is byte i * G + g of the lane's 4 G
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int at = i * G + g;
-      packed[at / 4] |= ((codes >> (8 * i)) & 0xffu) << (8 * (at % 4));
-    }
   }
+  interleave<G>(codes, packed);
   const uint64_t row = (uint64_t(page) * a.kv_heads + kv) * a.page_tokens + slot;
   uint8_t* dst = (is_v ? a.v : a.k) + row * (16u * G) + kg * (4u * G);
   if constexpr (G == 2) {
