@@ -20,11 +20,10 @@
 // any steps.  The blocks' values at code 8 add sum_t p_t mid_{t,g} in fp32.
 //
 // What bounds it: long contexts the cache's bytes (16 ragged sequences of up to
-// 32K tokens, 32 heads over 8 of dim 128: 77.5 us, 4.3 TB/s; four of 128K, 64
-// heads: 165 us, 4.1 TB/s; int8, 32 windows of 4,096, dim 256: 109.7 us, 4.6
-// TB/s), short ones the chain of dependent loads from the item to its pages, K
-// and the merge (512 tokens: 10 us), many head-rows of dim 256 the arithmetic of
-// a tile, 4 us of a wave with two on a SIMD (48 head-rows, 8K tokens: 34 us).
+// 32K tokens, 32 heads over 8 of dim 128: 76.7 us, 4.4 TB/s; four of 128K, 64
+// heads: 167 us, 4.0 TB/s; int8, 32 windows of 4,096, dim 256: 110 us, 4.6 TB/s), short ones the chain of dependent loads from the item to its pages, K
+// and the merge (512 tokens: 9.7 us), many head-rows of dim 256 the arithmetic of
+// a tile, 4 us of a wave with two on a SIMD (48 head-rows, 8K tokens: 33 us).
 #pragma once
 #include "scored.h"
 

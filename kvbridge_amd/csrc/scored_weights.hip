@@ -12,8 +12,9 @@
 // head-rows of a block is then a DPP reduction over every F-th lane of a row.
 //
 // What bounds it: 16 ragged sequences of up to 32K tokens (32 heads over 8, dim
-// 128) take 50 us, 3.7 TB/s of K and weights, the vector instructions of a tile
-// about 35 of them; plain stores in place of the atomics change nothing. Two
+// 128) take 50 us, 3.7 TB/s of K and weights: 4,400 vector instructions a wave are
+// 26 of them, and three waves a SIMD do not cover all waits for K; plain stores
+// in place of the atomics changed nothing (59.3 against 60.5 at the time).  Two
 // sequences of 7K under 64 head-rows of dim 64 over int8: 11 us, latency.
 #include "scored.h"
 
