@@ -223,7 +223,8 @@ int kvb_append_kv(const kvb_append_shape* s, const kvb_append_io* io, void* stre
  *      32g + 2n + 1.  k_scales / v_scales are G uint32 words per (page, kv
  *      head, slot), word g = the block's step as bfloat16 in the high half,
  *      its least value as bfloat16 in the low half: value = code * step + least.
- * Offsets into the pool are 64 bits wide: a pool may exceed 4 GiB. */
+ * Offsets into the pool are 64 bits wide: a pool may exceed 4 GiB.  Buffers and
+ * stream are the current device's. */
 enum { KVB_OUT_BF16 = 3 };
 
 /* Writes `tokens` new tokens' K and V rows into the 4-bit pool: the shape, the
@@ -275,8 +276,9 @@ int kvb_read_kv(const kvb_read_shape* s, const kvb_read_io* io, void* stream);
  * tokens; m = -inf, l = 0, out = 0 where there is none, or every s is -inf.
  * What masked tokens hold, NaN included, has no effect; in a visible token a
  * K scale or parameter that is not finite makes the row NaN, one of V the dims
- * that it enters, if the token's weight is not 0 in fp32.  Distances of 2^30
- * and more count as 2^30.  k_positions are nondecreasing within a sequence.
+ * that it enters, if the token's weight is not 0 in fp32.  With slopes, the
+ * positions of keys and rows count as at most 2^30 from the sequence's first
+ * row's.  k_positions are nondecreasing within a sequence.
  * q is [batch][rows][q_heads][dim] of q_type (KVB_SRC_*) with q_stride elements
  * from one row to the next.  split_tokens is a multiple of 32, or 0: up to 256
  * sequences then get items by their lengths, read on the device.  Q enters the

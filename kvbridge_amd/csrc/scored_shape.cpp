@@ -135,6 +135,11 @@ const char* evict_error(const kvb_evict_shape& s) {
   if (s.keep == 0 || s.keep > (1u << 30)) return "keep must be in [1,2^30]";
   if (uint64_t(s.sink) + s.recent > s.keep) return "sink and recent exceed keep";
   if (uint64_t(s.batch) * s.keep > 0xffffffffull) return "batch and keep product exceeds 32 bits";
+  // Work-groups of the two launches: 1,024 tokens, and 64 kept tokens of a kv head.
+  const uint64_t most = std::min(s.keep, s.max_tokens);
+  if (uint64_t(s.batch) * ceil_div(s.max_tokens, 1024) > 0x7fffffffull ||
+      uint64_t(s.batch) * s.kv_heads * ceil_div(most, 64) > 0x7fffffffull)
+    return "batch, tokens and heads exceed the grid limit";
   return nullptr;
 }
 

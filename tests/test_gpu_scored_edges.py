@@ -255,3 +255,24 @@ def test_head_rows_of_different_value_scales(gpu, bits, dim, heads, at):
     for split in (0, T):
         c.split_tokens = split
         check_attention(c, Attend(c, t, "f32")().read(), "f32")
+
+
+@pytest.mark.parametrize("bits,heads,dim", [(4, 4, 128), (4, 16, 64), (4, 4, 256), (8, 8, 128)])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_a_head_that_is_not_finite_stays_alone(gpu, bits, heads, dim, value):
+    """One query head with a NaN or an infinity: its own l and output are NaN, the
+    other heads of its kv head are as without it.  Their scores are the same; their
+    weights may be scaled at other tiles, 2^-19 of the largest value either way
+    (check_attention)."""
+    c = Case(bits, [900, 33], 1, heads, 1, dim, 16, seed=45, kind="f32")
+    t = c.to_device()
+    want = Attend(c, t, "f32")().read()
+    t["q"].view(2, heads, dim)[0, 1, 5] = value
+    got = Attend(c, t, "f32")().read()
+    keep = np.ones((2, 1, heads), bool)
+    keep[0, 0, 1] = False
+    assert np.array_equal(want[0][keep], got[0][keep])
+    assert np.all(np.abs(want[1] - got[1])[keep] <= 2.0 ** -19 * want[1][keep])
+    top = max(np.abs(c.rows_of(b, "v")).max() for b in range(2))
+    assert np.all(np.abs(want[2] - got[2])[keep] <= 2.0 ** -18 * top)
+    assert np.isnan(got[1][0, 0, 1]) and np.isnan(got[2][0, 0, 1]).all()
