@@ -13,8 +13,9 @@
 //
 // What bounds it: 16 ragged sequences of up to 32K tokens (32 heads over 8, dim
 // 128) take 50 us, 3.7 TB/s of K and weights: 4,400 vector instructions a wave are
-// 26 of them, and three waves a SIMD do not cover all waits for K; plain stores
-// in place of the atomics changed nothing (59.3 against 60.5 at the time).  Two
+// 26 of them, and three waves a SIMD do not cover all waits for K.  Neither K
+// requested two tiles ahead (49-50) nor plain stores in place of the atomics
+// (59.3 against 60.5 at the time) changed that.  Two
 // sequences of 7K under 64 head-rows of dim 64 over int8: 11 us, latency.
 #include "scored.h"
 
